@@ -23,6 +23,7 @@
 #include "../../include/needle_b200.h"
 #include "archive.h"
 #include "expf_table.h"
+#include "failure.h"
 #include "kernels.h"
 #include "layout.h"
 
@@ -32,38 +33,7 @@ namespace nbr {
 
 thread_local std::string g_error;
 
-struct Failure {
-  nb_status status;
-  std::string message;
-};
-
 [[noreturn]] void fail(nb_status s, const std::string& m) { throw Failure{s, m}; }
-
-#define NB_CUDA(call)                                                                                          \
-  do {                                                                                                         \
-    cudaError_t e_ = (call);                                                                                   \
-    if (e_ != cudaSuccess) ::nbr::fail(NB_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_));      \
-  } while (0)
-
-template <typename F>
-nb_status guard(F&& f) {
-  try {
-    f();
-    return NB_OK;
-  } catch (const Failure& e) {
-    g_error = e.message;
-    return e.status;
-  } catch (const nba::ArchiveError& e) {
-    g_error = e.message;
-    return (nb_status)e.status;
-  } catch (const std::bad_alloc&) {
-    g_error = "host allocation failed";
-    return NB_ERR_ARGUMENT;
-  } catch (const std::exception& e) {
-    g_error = e.what();
-    return NB_ERR_ARGUMENT;
-  }
-}
 
 // ------------------------------------------------------------ level tables
 // crates/kernels/src/codebook.rs:1-43 and matrix.rs:499-514
