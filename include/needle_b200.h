@@ -278,6 +278,152 @@ nb_status nb_build_expf_table(const char* path);
 nb_status nb_model_project_static(nb_model* model, int which, uint32_t layer, const float* in_device, uint32_t count,
                                   float* out_device, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Drafted decoding over a shared prompt: a quantised key/value cache that the
+ * caller fills and reads, attention of a whole batch over one prefix that
+ * every sequence shares and over each sequence's own tail, and the
+ * verification of drafted tokens. No reference counterpart: the reference
+ * decodes one sequence greedily, one token at a time (generator.rs:99-130),
+ * and shares a prefix only by cloning a Session (generator.rs:36-47).
+ *
+ * Every pointer in these calls is device memory of the cache's GPU (of
+ * `device` for nb_verify_drafts); `stream` is a cudaStream_t of that GPU, NULL
+ * its default stream. The calls queue their kernels on the stream and return;
+ * they allocate nothing, keep nothing between calls, may be recorded into a
+ * CUDA graph and leave the calling thread's current device as it was.
+ */
+
+typedef enum nb_dtype { NB_F32 = 0, NB_F16 = 1, NB_BF16 = 2 } nb_dtype;
+
+/* What a cache row holds: 8-bit codes and one f32 scale for every position and
+ * kv head, for keys and for values.
+ * NB_KV_INT8: scale = peak * (1/127), both in f32 (peak = the row's largest
+ *   magnitude), code = x / scale rounded to the nearest integer, halves to even.
+ * NB_KV_E4M3: scale = the smallest power of two s with peak <= 448 s, code =
+ *   x / s rounded to e4m3 (nearest, halves to even).
+ * A row of zeros has scale 1. No scale is below 2^-60: rows of smaller numbers
+ * lose their low bits. A row with a NaN, an infinity or a
+ * magnitude above 2^40 is held as NaN as a whole, and reads so. */
+typedef enum nb_kv_format { NB_KV_INT8 = 0, NB_KV_E4M3 = 1 } nb_kv_format;
+
+#define NB_KV_PAGE 64u /* positions of a page */
+
+typedef struct nb_kv_cache nb_kv_cache;
+
+/* A pool of `pages` pages of NB_KV_PAGE positions, each with kv_heads (1..256)
+ * keys and values of head_dim (64 or 128) codes, on GPU `device` (-1 = the
+ * current device). Which sequence owns which page is the caller's to say, in
+ * every call. NB_ERR_CUDA when the memory is not to be had. */
+nb_status nb_kv_cache_create(int32_t device, int32_t format, uint32_t kv_heads, uint32_t head_dim, uint32_t pages,
+                             nb_kv_cache** out);
+/* Waits for the GPU's running work and frees the pool. */
+void nb_kv_cache_release(nb_kv_cache* cache);
+
+/* The sequences of a call and their rows. Sequence b has the rows
+ * row_start[b] .. row_start[b + 1] of the dense buffers, n of them (0 to
+ * max_rows), and lengths[b] cached positions, of which its rows are the last
+ * n: row i stands at position lengths[b] - n + i. Position p lies in page
+ * pages[b * page_stride + p / NB_KV_PAGE]. rows, max_rows and max_length bound
+ * row_start[sequences], n and lengths[b]; they size the launches, so close
+ * bounds are faster. The arrays are device memory and may change between
+ * replays of a graph, within those bounds. A sequence that breaks a bound
+ * (or has lengths[b] < n, or lengths[b] > page_stride * NB_KV_PAGE) is left
+ * out: nothing of it is written. A page number outside the pool is neither
+ * read (its positions count as masked) nor written. nb_kv_cache_check reports
+ * both. Rows of the buffers that belong to no sequence are left as they were. */
+typedef struct nb_kv_batch {
+  uint32_t sequences, rows, max_rows, max_length;
+  uint32_t page_stride;
+  const int32_t* row_start; /* sequences + 1 */
+  const int32_t* lengths;   /* sequences */
+  const uint32_t* pages;    /* sequences x page_stride */
+} nb_kv_batch;
+
+/* A dense buffer [rows][heads][head_dim] of nb_dtype `dtype`; head_dim is
+ * contiguous, the other strides are in elements and not negative. An output's
+ * rows and heads must not overlap. */
+typedef struct nb_rows {
+  void* data;
+  int32_t dtype;
+  int64_t row_stride, head_stride;
+} nb_rows;
+
+/* Quantises the batch's rows of keys and values ([rows][kv_heads][head_dim])
+ * into the cache, at their positions. A page that several sequences share may
+ * be read by all but written by one: where two rows of a call fall on the same
+ * position of the same page, which of them is kept is not specified, not even
+ * code by code. */
+nb_status nb_kv_cache_append(nb_kv_cache* cache, const nb_kv_batch* batch, const nb_rows* keys, const nb_rows* values, void* stream);
+
+/* Reads the batch's rows back into keys and values: code x scale, rounded once
+ * to the buffer's type. Rows in a page outside the pool are left as they were. */
+nb_status nb_kv_cache_read(const nb_kv_cache* cache, const nb_kv_batch* batch, const nb_rows* keys, const nb_rows* values, void* stream);
+
+/* Bytes of workspace that nb_kv_cache_attend needs for these bounds. */
+nb_status nb_kv_cache_attend_workspace(const nb_kv_cache* cache, const nb_kv_batch* batch, uint32_t prefix_length, uint32_t heads,
+                                       size_t* bytes);
+
+/* Attention of the batch's rows. Query row i of sequence b (position
+ * lengths[b] - n + i of its tail), head h reads kv head h / (heads / kv_heads)
+ * and attends to all prefix_length positions of the shared prefix (whose
+ * position p lies in page prefix_pages[p / NB_KV_PAGE]; prefix_length 0: no
+ * prefix) and to the positions 0 .. lengths[b] - n + i of its own tail:
+ *   out = sum_j softmax_j(scale * q.k_j) v_j,
+ * with k_j and v_j the values that the cache holds. A row without any visible
+ * position (its pages outside the pool) gets zeros. query and out are
+ * [rows][heads][head_dim], both NB_F16 or both NB_BF16; heads is a multiple of
+ * kv_heads, at most 64 for each. The prefix is read once for the whole batch.
+ * The tail's new rows have to be in the cache (nb_kv_cache_append, earlier on
+ * the same stream). Sums, maxima and products are accumulated in f32; the
+ * probabilities enter their product with the codes as f16. `workspace` is
+ * 16-byte aligned, nb_kv_cache_attend_workspace bytes, free for other use once
+ * the call's kernels are done; calls that may overlap (two streams, two graphs)
+ * need one each. */
+nb_status nb_kv_cache_attend(const nb_kv_cache* cache, const nb_kv_batch* batch, const uint32_t* prefix_pages, uint32_t prefix_length,
+                             const nb_rows* query, const nb_rows* out, uint32_t heads, float scale, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Waits for the stream and reports NB_ERR_ARGUMENT if a call on this cache met
+ * a sequence out of its bounds or a page outside the pool since the last
+ * check, NB_ERR_TIMEOUT if a bounded device wait gave up; clears the report. */
+nb_status nb_kv_cache_check(nb_kv_cache* cache, void* stream);
+
+/* Drafted tokens against the target model. Sequence b has draft_counts[b]
+ * drafted tokens (clamped to 0..drafts; NULL: all of them) and one row of
+ * target logits for each and one more for the place behind the last: row i of
+ * sequence b starts at logits + (b * (drafts + 1) + i) * row_stride elements. */
+typedef struct nb_verify {
+  uint32_t sequences, drafts, vocab;
+  int32_t dtype;      /* of logits: nb_dtype */
+  int64_t row_stride; /* elements, >= vocab */
+  const void* logits;
+  const float* draft_probabilities; /* [sequences][drafts][vocab], or NULL: every draft was certain (probability 1) */
+  const uint32_t* draft_tokens;     /* [sequences][drafts] */
+  const int32_t* draft_counts;      /* [sequences], or NULL */
+  const uint32_t* mask_bits;        /* [sequences][drafts + 1][(vocab + 31) / 32] allowed ids (nb_batch_step's layout), or NULL */
+  const float* accept_uniforms;     /* [sequences][drafts], in [0, 1) */
+  const float* sample_uniforms;     /* [sequences], in [0, 1) */
+  float temperature;                /* >= 0 */
+  uint32_t* tokens;                 /* out: [sequences][drafts + 1] */
+  int32_t* accepted;                /* out: [sequences] */
+} nb_verify;
+
+/* For i = 0, 1, ..: with p = softmax(logits_i / temperature) over the allowed
+ * ids (all ids, if the mask allows none: generator.rs:147-155) and q =
+ * draft_probabilities_i, the drafted token d is accepted while
+ * accept_uniform_i * q(d) < p(d). At the first rejection the token is drawn
+ * from max(p - q, 0), behind the last accepted draft from p: the lowest id
+ * whose running sum passes sample_uniform * total. Where p nowhere exceeds q
+ * the draw is from p. So the tokens are distributed as the target's own.
+ * temperature 0: a draft is accepted while it is the allowed argmax (lowest id
+ * on ties), which else takes its place; the random numbers and q are not read.
+ * accepted[b] is the number of accepted drafts; tokens[b] are these, the drawn
+ * token, then UINT32_MAX. A NaN logit counts as -inf and +inf as the largest
+ * float; a row with nothing left but -inf accepts nothing and draws
+ * UINT32_MAX. A drafted id outside the vocabulary is never accepted. The
+ * probabilities and running sums that decide a draw are formed in 64 bits. */
+nb_status nb_verify_drafts(int32_t device, const nb_verify* verify, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

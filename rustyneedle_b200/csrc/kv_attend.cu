@@ -1,0 +1,382 @@
+// kv_attend.cu — attention of a batch over one shared prefix and over each
+// sequence's own tail, on the 8-bit paged cache.
+//
+// With K_j = ks_j · kc_j and V_j = vs_j · vc_j (codes kc, vc; f32 scales ks, vs)
+//   t_j = (q·kc_j) · ks_j · scale · log2 e + log2 vs_j      w_j = 2^(t_j - m)
+//   out = Σ w_j vc_j / Σ w_j / vs_j
+// so the codes enter both products exactly and every scale stays in f32: the
+// value scale is folded into the exponent, and dividing it out again gives the
+// softmax's own sum. m is the running maximum of t less HEADROOM, so w_j ≤
+// 2^HEADROOM; the product with the codes takes w as f16 (2^-12 relative down
+// to 2^-14, absolute 2^-25 below), the sums take it as f32.
+#include "serving.cuh"
+
+namespace nbk {
+
+constexpr float HEADROOM = 8.0f;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct AttendDev {
+  KvCacheDev c;
+  KvBatchDev b;
+  const uint32_t* prefix_pages;
+  int prefix, heads, group;
+  float scale;  // softmax scale · log2 e
+  RowsDev q, out;
+  bool q_vector;
+  float* part_o;  // [parts][rows][heads][dim], unnormalised
+  float2* part_ml;  // [parts][rows][heads]: maximum (less HEADROOM) and sum
+  int prefix_parts, tail_parts;
+  int prefix_chunk, tail_chunk;  // keys of a part, multiples of 32
+  int tiles_per_sequence;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 16 query rows of one kv head against a part of the prefix (PREFIX) or of a
+// sequence's tail. A row is (token, query head of the group): row r of a tile
+// list stands for token r / group. Four warps take the part's keys 32 at a
+// time in turn and are joined at the end.
+//
+// Lanes: g = lane / 4, c = lane % 4. The key fragment of a 16 x 8 x 16 product
+// wants, of key "n = g", four dimensions of the lane's own choice for every
+// step, as long as the query fragment has the same: lane c takes 16
+// consecutive bytes of every 64, four steps of four dimensions, so a key's
+// codes arrive as one 16-byte load and need no shared memory. Product j of a
+// block of 16 keys takes the keys 4·(n / 2) + 2·j + n % 2, which leaves lane c
+// the scores of the keys 4c .. 4c + 3: the order in which the second product
+// wants its left operand, and in which the pool keeps the values (value_byte).
+constexpr int ATT_WARPS = 4;
+
+template <int D, bool BF16, bool E4M3, bool PREFIX>
+__global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a) {
+  constexpr int SEG = D / 64, STEPS = D / 16, NT = D / 8;
+  __shared__ float s_o[ATT_WARPS][16][D + 1];
+  __shared__ float2 s_ml[ATT_WARPS][16];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int h = blockIdx.y, part = blockIdx.z;
+  int token0, tokens, row0, k0, k1, sees0 = 0;  // the tile's rows row0.. of `tokens` tokens from token0; keys [k0, k1)
+  const uint32_t* pages;
+  if constexpr (PREFIX) {
+    row0 = blockIdx.x * 16;
+    token0 = 0;
+    tokens = a.b.rows;
+    k0 = part * a.prefix_chunk;
+    k1 = min(a.prefix, k0 + a.prefix_chunk);
+    pages = a.prefix_pages;
+  } else {
+    const int s = blockIdx.x / a.tiles_per_sequence;
+    row0 = (blockIdx.x % a.tiles_per_sequence) * 16;
+    const Span sp = span_of(a.b, s);
+    if (!sp.ok) {
+      if (threadIdx.x == 0) atomicOr(a.c.error, KV_BAD_SEQUENCE);
+      return;
+    }
+    token0 = sp.first;
+    tokens = sp.n;
+    if (row0 >= tokens * a.group) return;
+    sees0 = sp.len - sp.n;
+    k0 = part * a.tail_chunk;
+    k1 = min(sees0 + min(tokens - 1, (row0 + 15) / a.group) + 1, k0 + a.tail_chunk);
+    pages = a.b.pages + (size_t)s * a.b.page_stride;
+  }
+  const int rows = tokens * a.group;
+
+  // the lane's query fragments; rows past the end are zeros
+  uint32_t qf[STEPS][4];
+  int limit[2];  // keys below it are seen by rows g and g + 8
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = row0 + g + 8 * half;
+    const bool live = r < rows;
+    const int token = live ? r / a.group : 0;
+    limit[half] = PREFIX ? k1 : min(k1, sees0 + token + 1);
+    const uint16_t* src = static_cast<const uint16_t*>(a.q.data) + (token0 + token) * a.q.row_stride +
+                          (h * a.group + (live ? r % a.group : 0)) * a.q.head_stride;
+#pragma unroll
+    for (int seg = 0; seg < SEG; ++seg)
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        uint2 x = make_uint2(0, 0);
+        if (live) {
+          const uint16_t* p = src + seg * 64 + c * 16 + st * 4;
+          if (a.q_vector) {
+            x = *reinterpret_cast<const uint2*>(p);
+          } else {
+            x.x = p[0] | (uint32_t)p[1] << 16;
+            x.y = p[2] | (uint32_t)p[3] << 16;
+          }
+        }
+        qf[seg * 4 + st][half] = x.x;
+        qf[seg * 4 + st][2 + half] = x.y;
+      }
+  }
+
+  float o[NT][4] = {};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  for (int kb = k0 + 32 * warp; kb < k1; kb += 32 * ATT_WARPS) {
+    const uint32_t page = pages[kb / KV_PAGE];
+    if (page >= a.c.pages) {
+      if (lane == 0) atomicOr(a.c.error, KV_BAD_PAGE);
+      continue;
+    }
+    const size_t block = (size_t)page * a.c.kv_heads + h;
+    const int in_page = kb % KV_PAGE;
+    const uint8_t* kp = a.c.k + block * (KV_PAGE * D) + in_page * D;
+    const uint8_t* vp = a.c.v + block * (KV_PAGE * D) + in_page * D;
+    float t[2][2][4];  // [block of 16 keys][product][row g: two keys, row g + 8: two keys]
+    float inv[2][4];   // 1 / vs of the keys 4c .. 4c + 3
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      const float4 ks = *reinterpret_cast<const float4*>(a.c.ks + block * KV_PAGE + in_page + blk * 16 + c * 4);
+      const float4 vs = *reinterpret_cast<const float4*>(a.c.vs + block * KV_PAGE + in_page + blk * 16 + c * 4);
+      const float kscale[4] = {ks.x, ks.y, ks.z, ks.w}, vscale[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float s[4] = {};
+        const uint8_t* row = kp + (blk * 16 + 4 * (g >> 1) + 2 * j + (g & 1)) * D + c * 16;
+#pragma unroll
+        for (int seg = 0; seg < SEG; ++seg) {
+          const uint4 w = *reinterpret_cast<const uint4*>(row + seg * 64);
+          const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int st = 0; st < 4; ++st) {
+            const uint2 kf = widen<E4M3, BF16>(word[st]);
+            mma16816<BF16>(s, qf[seg * 4 + st], kf.x, kf.y);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int e = 2 * j + i, key = kb + blk * 16 + 4 * c + e;
+          const float mul = __fmul_rn(kscale[e], a.scale), add = lg2(vscale[e]);
+          inv[blk][e] = key < k1 ? __frcp_rn(vscale[e]) : 0.0f;
+          // a key that a row does not see gets -inf by selection, whatever lies there
+          t[blk][j][i] = key < limit[0] ? __fmaf_rn(s[i], mul, add) : -INFINITY;
+          t[blk][j][2 + i] = key < limit[1] ? __fmaf_rn(s[2 + i], mul, add) : -INFINITY;
+        }
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(t[blk][j][2 * half], t[blk][j][2 * half + 1]));
+      top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+      const float next = fmaxf(m[half], __fadd_rn(top, -HEADROOM));
+      const float base = next == -INFINITY ? 0.0f : next;
+      const float keep = ex2(__fadd_rn(m[half], -base));  // 0 while nothing was seen
+      m[half] = next;
+      float sum = 0.0f;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float& x = t[blk][j][2 * half + i];
+            const bool seen = x != -INFINITY;
+            x = ex2(__fadd_rn(x, -base));
+            sum = seen ? __fmaf_rn(x, inv[blk][2 * j + i], sum) : sum;
+          }
+      l[half] = __fmaf_rn(l[half], keep, sum);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        o[n][2 * half] = __fmul_rn(o[n][2 * half], keep);
+        o[n][2 * half + 1] = __fmul_rn(o[n][2 * half + 1], keep);
+      }
+    }
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      const uint32_t pf[4] = {pack_f16(t[blk][0][0], t[blk][0][1]), pack_f16(t[blk][0][2], t[blk][0][3]), pack_f16(t[blk][1][0], t[blk][1][1]),
+                              pack_f16(t[blk][1][2], t[blk][1][3])};
+#pragma unroll
+      for (int tq = 0; tq < D / 32; ++tq) {
+        const uint4 w = *reinterpret_cast<const uint4*>(vp + blk * 16 * D + tq * 512 + g * 64 + c * 16);
+        const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint2 vf = widen<E4M3, false>(word[n]);
+          mma16816<false>(o[tq * 4 + n], pf, vf.x, vf.y);
+        }
+      }
+    }
+  }
+
+  // join the four warps: rows of a common maximum
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    l[half] = __fadd_rn(l[half], __shfl_xor_sync(FULL, l[half], 1));
+    l[half] = __fadd_rn(l[half], __shfl_xor_sync(FULL, l[half], 2));
+    if (c == 0) s_ml[warp][g + 8 * half] = make_float2(m[half], l[half]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      s_o[warp][g + 8 * half][n * 8 + 2 * c] = o[n][2 * half];
+      s_o[warp][g + 8 * half][n * 8 + 2 * c + 1] = o[n][2 * half + 1];
+    }
+  }
+  __syncthreads();
+  const int index = PREFIX ? part : a.prefix_parts + part;
+  for (int x = threadIdx.x; x < 16 * D; x += ATT_WARPS * 32) {
+    const int r = x / D, d = x % D;
+    if (row0 + r >= rows) break;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < ATT_WARPS; ++w) top = fmaxf(top, s_ml[w][r].x);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, value = 0.0f;
+#pragma unroll
+    for (int w = 0; w < ATT_WARPS; ++w) {
+      const float f = ex2(__fadd_rn(s_ml[w][r].x, -base));
+      sum = __fmaf_rn(s_ml[w][r].y, f, sum);
+      value = __fmaf_rn(s_o[w][r][d], f, value);
+    }
+    const size_t at = ((size_t)index * a.b.rows + token0 + (row0 + r) / a.group) * a.heads + h * a.group + (row0 + r) % a.group;
+    a.part_o[at * D + d] = value;
+    if (d == 0) a.part_ml[at] = make_float2(top, sum);
+  }
+}
+
+// Joins the parts of a row: one warp for each (token, head).
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) k_kv_join(AttendDev a) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x & 31;
+  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit >= (long long)a.b.rows * a.heads) return;
+  const int row = (int)(unit / a.heads), head = (int)(unit % a.heads);
+  const int s = sequence_of(a.b, row);
+  const Span sp = span_of(a.b, s);
+  if (!sp.ok || row < sp.first || row >= sp.first + sp.n) return;
+  const int parts = a.prefix_parts + a.tail_parts;
+  const size_t stride = (size_t)a.b.rows * a.heads;
+  float top = -INFINITY;
+  for (int p = 0; p < parts; ++p) top = fmaxf(top, a.part_ml[p * stride + unit].x);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f, x[N] = {};
+  for (int p = 0; p < parts; ++p) {
+    const float2 ml = a.part_ml[p * stride + unit];
+    const float f = ex2(__fadd_rn(ml.x, -base));
+    sum = __fmaf_rn(ml.y, f, sum);
+    const float* o = a.part_o + (p * stride + unit) * D + lane * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(o[i], f, x[i]);
+  }
+  const float norm = sum == 0.0f ? 0.0f : __frcp_rn(sum);
+  const long long at = row * a.out.row_stride + head * a.out.head_stride + lane * N;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float y = __fmul_rn(x[i], norm);
+    if constexpr (BF16)
+      static_cast<__nv_bfloat16*>(a.out.data)[at + i] = __float2bfloat16_rn(y);
+    else
+      static_cast<__half*>(a.out.data)[at + i] = __float2half_rn(y);
+  }
+}
+
+// How the keys are split into parts: enough CTAs for the 148 SMs, parts of at
+// least 128 keys. The same plan sizes the workspace.
+struct AttendPlan {
+  int prefix_parts = 0, prefix_chunk = 0, tail_parts = 1, tail_chunk = 0, tiles_per_sequence = 1;
+};
+
+static AttendPlan attend_plan(const KvCacheDev& c, const KvBatchDev& b, int prefix, int heads) {
+  AttendPlan p;
+  const int group = heads / c.kv_heads;
+  auto split = [](int keys, long long tiles, int* parts, int* chunk) {
+    *parts = 0;
+    *chunk = 32;
+    if (keys == 0 || tiles == 0) return;
+    const long long want = (4 * 148 + tiles - 1) / tiles;
+    const int most = (keys + 127) / 128;
+    const int n = (int)(want > most ? most : want);
+    *chunk = (((keys + n - 1) / n) + 31) / 32 * 32;
+    *parts = (keys + *chunk - 1) / *chunk;
+  };
+  split(prefix, ((long long)b.rows * group + 15) / 16 * c.kv_heads, &p.prefix_parts, &p.prefix_chunk);
+  p.tiles_per_sequence = (int)(((long long)b.max_rows * group + 15) / 16);
+  if (p.tiles_per_sequence < 1) p.tiles_per_sequence = 1;
+  split(b.max_length, (long long)b.sequences * p.tiles_per_sequence * c.kv_heads, &p.tail_parts, &p.tail_chunk);
+  return p;
+}
+
+size_t kv_attend_workspace(const KvCacheDev& c, const KvBatchDev& b, int prefix, int heads) {
+  const AttendPlan p = attend_plan(c, b, prefix, heads);
+  const size_t units = (size_t)(p.prefix_parts + p.tail_parts) * b.rows * heads;
+  return units * (c.dim * sizeof(float) + sizeof(float2)) + 16;
+}
+
+template <int D, bool BF16, bool E4M3>
+static cudaError_t attend_launch(const AttendDev& d, cudaStream_t st) {
+  if (d.prefix_parts) {
+    const dim3 grid((unsigned)(((long long)d.b.rows * d.group + 15) / 16), d.c.kv_heads, d.prefix_parts);
+    k_kv_attend<D, BF16, E4M3, true><<<grid, ATT_WARPS * 32, 0, st>>>(d);
+  }
+  if (d.tail_parts) {
+    const dim3 grid((unsigned)d.b.sequences * d.tiles_per_sequence, d.c.kv_heads, d.tail_parts);
+    k_kv_attend<D, BF16, E4M3, false><<<grid, ATT_WARPS * 32, 0, st>>>(d);
+  }
+  k_kv_join<D, BF16><<<(unsigned)(((long long)d.b.rows * d.heads + 7) / 8), 256, 0, st>>>(d);
+  return cudaGetLastError();
+}
+
+cudaError_t kv_attend(const KvCacheDev& c, const KvBatchDev& b, const KvAttend& x, cudaStream_t st) {
+  if (b.sequences == 0 || b.rows == 0) return cudaSuccess;
+  const AttendPlan p = attend_plan(c, b, x.prefix, x.heads);
+  AttendDev d;
+  d.c = c;
+  d.b = b;
+  d.prefix_pages = x.prefix_pages;
+  d.prefix = x.prefix;
+  d.heads = x.heads;
+  d.group = x.heads / c.kv_heads;
+  d.scale = x.scale * LOG2E;
+  d.q = x.query;
+  d.out = x.out;
+  d.q_vector = reinterpret_cast<uintptr_t>(x.query.data) % 8 == 0 && x.query.row_stride % 4 == 0 && x.query.head_stride % 4 == 0;
+  d.prefix_parts = p.prefix_parts;
+  d.prefix_chunk = p.prefix_chunk;
+  d.tail_parts = p.tail_parts;
+  d.tail_chunk = p.tail_chunk;
+  d.tiles_per_sequence = p.tiles_per_sequence;
+  const size_t units = (size_t)(p.prefix_parts + p.tail_parts) * b.rows * x.heads;
+  d.part_o = static_cast<float*>(x.workspace);
+  d.part_ml = reinterpret_cast<float2*>(d.part_o + units * c.dim);
+  const bool bf16 = x.query.dtype == DTYPE_BF16;
+  if (c.dim == 64) {
+    if (bf16) return c.e4m3 ? attend_launch<64, true, true>(d, st) : attend_launch<64, true, false>(d, st);
+    return c.e4m3 ? attend_launch<64, false, true>(d, st) : attend_launch<64, false, false>(d, st);
+  }
+  if (bf16) return c.e4m3 ? attend_launch<128, true, true>(d, st) : attend_launch<128, true, false>(d, st);
+  return c.e4m3 ? attend_launch<128, false, true>(d, st) : attend_launch<128, false, false>(d, st);
+}
+
+}  // namespace nbk
