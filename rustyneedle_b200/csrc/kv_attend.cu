@@ -9,43 +9,9 @@
 // softmax's own sum. m is the running maximum of t less HEADROOM, so w_j ≤
 // 2^HEADROOM; the product with the codes takes w as f16 (2^-12 relative down
 // to 2^-14, absolute 2^-25 below), the sums take it as f32.
-#include "serving.cuh"
+#include "kv_attend.cuh"
 
 namespace nbk {
-
-constexpr float HEADROOM = 8.0f;
-constexpr float LOG2E = 1.4426950408889634f;
-
-struct AttendDev {
-  KvCacheDev c;
-  KvBatchDev b;
-  const uint32_t* prefix_pages;
-  int prefix, heads, group;
-  float scale;  // softmax scale · log2 e
-  RowsDev q, out;
-  bool q_vector;
-  float* part_o;  // [parts][rows][heads][dim], unnormalised
-  float2* part_ml;  // [parts][rows][heads]: maximum (less HEADROOM) and sum
-  int prefix_parts, tail_parts;
-  int prefix_chunk, tail_chunk;  // keys of a part, multiples of 32
-  int tiles_per_sequence;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -302,48 +268,88 @@ __global__ void __launch_bounds__(256) k_kv_join(AttendDev a) {
   }
 }
 
-// How the keys are split into parts: enough CTAs for the 148 SMs, parts of at
-// least 128 keys. The same plan sizes the workspace.
+// How a side (the prefix or the tails) is cut: the kernel, its row tiles and
+// its chunks of keys. The same plan sizes the workspace.
+struct SidePlan {
+  bool wide = false, pair = false;
+  int tiles = 0;   // row tiles (prefix: of the batch, tails: of a sequence)
+  int chunks = 0;  // of keys
+  int chunk = 32, parts = 0;
+};
+
+constexpr int WIDE_FROM = 33;  // rows that meet the same keys
+
+// rows: query rows (token, head of the group) that meet the same `keys`;
+// `lists`: how many such sets there are (kv heads, times sequences).
+static SidePlan side_plan(long long rows, int keys, long long lists, size_t part_bytes) {
+  SidePlan p;
+  p.wide = rows >= WIDE_FROM;
+  p.pair = rows > 128;
+  const int cover = p.wide ? (p.pair ? 256 : 128) : 16, unit = p.wide ? 128 : 32;
+  p.tiles = (int)((rows + cover - 1) / cover);
+  if (keys == 0 || lists == 0 || p.tiles == 0) return p;
+  const int units = (keys + unit - 1) / unit;
+  int chunks = 1;
+  if (p.wide) {
+    // one CTA an SM: the fewest rounds of key tiles, with the time of a tile
+    // (about 1 us) against that of writing and joining one more part
+    double best = 0;
+    for (int n = 1; n <= units && n <= 64; ++n) {
+      const long long rounds = (lists * p.tiles * n + 147) / 148;
+      const double cost = (double)rounds * ((units + n - 1) / n + 2) + (double)n * (p.pair ? 1 : 2) * part_bytes * 2 / 4e6;
+      if (n == 1 || cost < best) {
+        best = cost;
+        chunks = n;
+      }
+    }
+  } else {
+    // small CTAs, about four an SM, of at least 128 keys
+    const long long want = (4 * 148 + lists * p.tiles - 1) / (lists * p.tiles);
+    chunks = (int)(want > (units + 3) / 4 ? (units + 3) / 4 : want);
+  }
+  const int each = (units + chunks - 1) / chunks;
+  p.chunk = each * unit;
+  p.chunks = (units + each - 1) / each;
+  p.parts = p.chunks * (p.wide && !p.pair ? 2 : 1);
+  return p;
+}
+
 struct AttendPlan {
-  int prefix_parts = 0, prefix_chunk = 0, tail_parts = 1, tail_chunk = 0, tiles_per_sequence = 1;
+  SidePlan prefix, tail;
 };
 
 static AttendPlan attend_plan(const KvCacheDev& c, const KvBatchDev& b, int prefix, int heads) {
+  const long long group = heads / c.kv_heads;
+  const size_t part_bytes = (size_t)b.rows * heads * c.dim * sizeof(float);
   AttendPlan p;
-  const int group = heads / c.kv_heads;
-  auto split = [](int keys, long long tiles, int* parts, int* chunk) {
-    *parts = 0;
-    *chunk = 32;
-    if (keys == 0 || tiles == 0) return;
-    const long long want = (4 * 148 + tiles - 1) / tiles;
-    const int most = (keys + 127) / 128;
-    const int n = (int)(want > most ? most : want);
-    *chunk = (((keys + n - 1) / n) + 31) / 32 * 32;
-    *parts = (keys + *chunk - 1) / *chunk;
-  };
-  split(prefix, ((long long)b.rows * group + 15) / 16 * c.kv_heads, &p.prefix_parts, &p.prefix_chunk);
-  p.tiles_per_sequence = (int)(((long long)b.max_rows * group + 15) / 16);
-  if (p.tiles_per_sequence < 1) p.tiles_per_sequence = 1;
-  split(b.max_length, (long long)b.sequences * p.tiles_per_sequence * c.kv_heads, &p.tail_parts, &p.tail_chunk);
+  p.prefix = side_plan(b.rows * group, prefix, c.kv_heads, part_bytes);
+  p.tail = side_plan(b.max_rows * group, b.max_length, (long long)b.sequences * c.kv_heads, part_bytes);
   return p;
 }
 
 size_t kv_attend_workspace(const KvCacheDev& c, const KvBatchDev& b, int prefix, int heads) {
   const AttendPlan p = attend_plan(c, b, prefix, heads);
-  const size_t units = (size_t)(p.prefix_parts + p.tail_parts) * b.rows * heads;
+  const size_t units = (size_t)(p.prefix.parts + p.tail.parts) * b.rows * heads;
   return units * (c.dim * sizeof(float) + sizeof(float2)) + 16;
 }
 
 template <int D, bool BF16, bool E4M3>
-static cudaError_t attend_launch(const AttendDev& d, cudaStream_t st) {
-  if (d.prefix_parts) {
-    const dim3 grid((unsigned)(((long long)d.b.rows * d.group + 15) / 16), d.c.kv_heads, d.prefix_parts);
-    k_kv_attend<D, BF16, E4M3, true><<<grid, ATT_WARPS * 32, 0, st>>>(d);
+static cudaError_t attend_launch(const AttendDev& d, const AttendPlan& p, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
+  if (p.prefix.chunks) {
+    if (p.prefix.wide)
+      e = attend_wide(d, true, p.prefix.tiles, p.prefix.chunks, st);
+    else
+      k_kv_attend<D, BF16, E4M3, true><<<dim3(p.prefix.tiles, d.c.kv_heads, p.prefix.chunks), ATT_WARPS * 32, 0, st>>>(d);
   }
-  if (d.tail_parts) {
-    const dim3 grid((unsigned)d.b.sequences * d.tiles_per_sequence, d.c.kv_heads, d.tail_parts);
-    k_kv_attend<D, BF16, E4M3, false><<<grid, ATT_WARPS * 32, 0, st>>>(d);
+  if (e == cudaSuccess && p.tail.chunks) {
+    const unsigned tiles = (unsigned)d.b.sequences * p.tail.tiles;
+    if (p.tail.wide)
+      e = attend_wide(d, false, (int)tiles, p.tail.chunks, st);
+    else
+      k_kv_attend<D, BF16, E4M3, false><<<dim3(tiles, d.c.kv_heads, p.tail.chunks), ATT_WARPS * 32, 0, st>>>(d);
   }
+  if (e != cudaSuccess) return e;
   k_kv_join<D, BF16><<<(unsigned)(((long long)d.b.rows * d.heads + 7) / 8), 256, 0, st>>>(d);
   return cudaGetLastError();
 }
@@ -362,21 +368,24 @@ cudaError_t kv_attend(const KvCacheDev& c, const KvBatchDev& b, const KvAttend& 
   d.q = x.query;
   d.out = x.out;
   d.q_vector = reinterpret_cast<uintptr_t>(x.query.data) % 8 == 0 && x.query.row_stride % 4 == 0 && x.query.head_stride % 4 == 0;
-  d.prefix_parts = p.prefix_parts;
-  d.prefix_chunk = p.prefix_chunk;
-  d.tail_parts = p.tail_parts;
-  d.tail_chunk = p.tail_chunk;
-  d.tiles_per_sequence = p.tiles_per_sequence;
-  const size_t units = (size_t)(p.prefix_parts + p.tail_parts) * b.rows * x.heads;
+  d.q_vector16 = reinterpret_cast<uintptr_t>(x.query.data) % 16 == 0 && x.query.row_stride % 8 == 0 && x.query.head_stride % 8 == 0;
+  d.prefix_parts = p.prefix.parts;
+  d.prefix_chunk = p.prefix.chunk;
+  d.prefix_pair = p.prefix.pair;
+  d.tail_parts = p.tail.parts;
+  d.tail_chunk = p.tail.chunk;
+  d.tail_pair = p.tail.pair;
+  d.tiles_per_sequence = p.tail.tiles;
+  const size_t units = (size_t)(p.prefix.parts + p.tail.parts) * b.rows * x.heads;
   d.part_o = static_cast<float*>(x.workspace);
   d.part_ml = reinterpret_cast<float2*>(d.part_o + units * c.dim);
   const bool bf16 = x.query.dtype == DTYPE_BF16;
   if (c.dim == 64) {
-    if (bf16) return c.e4m3 ? attend_launch<64, true, true>(d, st) : attend_launch<64, true, false>(d, st);
-    return c.e4m3 ? attend_launch<64, false, true>(d, st) : attend_launch<64, false, false>(d, st);
+    if (bf16) return c.e4m3 ? attend_launch<64, true, true>(d, p, st) : attend_launch<64, true, false>(d, p, st);
+    return c.e4m3 ? attend_launch<64, false, true>(d, p, st) : attend_launch<64, false, false>(d, p, st);
   }
-  if (bf16) return c.e4m3 ? attend_launch<128, true, true>(d, st) : attend_launch<128, true, false>(d, st);
-  return c.e4m3 ? attend_launch<128, false, true>(d, st) : attend_launch<128, false, false>(d, st);
+  if (bf16) return c.e4m3 ? attend_launch<128, true, true>(d, p, st) : attend_launch<128, true, false>(d, p, st);
+  return c.e4m3 ? attend_launch<128, false, true>(d, p, st) : attend_launch<128, false, false>(d, p, st);
 }
 
 }  // namespace nbk

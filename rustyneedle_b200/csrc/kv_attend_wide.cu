@@ -1,0 +1,465 @@
+// kv_attend_wide.cu — the shared-prefix attention where many query rows meet
+// the same keys (the prefix of a batch, the tails of long questions): tiles of
+// 128 rows on the tcgen05 tensor cores.
+//
+// A CTA holds two slots, each an accumulator of 128 rows:
+//   two tiles: the slots are two row tiles and share every key tile, so the
+//              8-bit codes are widened once for 256 rows;
+//   one tile:  the slots are one row tile over alternate key tiles.
+// While one slot's scores go through the softmax, the tensor cores work for
+// the other. Warps 0-3 and 4-7 are the slots' softmax (a thread is a row:
+// TMEM lane = row), warps 8-11 load codes and widen them into shared memory,
+// one lane of warp 12 issues the matrix instructions:
+//   S = Q K^T   Q and K codes (f16 or bf16) from shared memory, f32 in TMEM
+//   O += P V    P (f16) from TMEM, over the first half of S; V codes (f16)
+// O is rescaled in TMEM only when a row's maximum has grown by more than
+// SLACK: until then the weights just get larger, up to 2^(HEADROOM + SLACK).
+//
+// Per 128 keys and slot: 4 · 128 · 128 · D flops on the tensor cores (512
+// cycles at D = 64, 1024 at D = 128), 16384 exponentials (1024 cycles of the
+// special-function units), so at D = 64 the exponentials bound the kernel and
+// at D = 128 both are even.
+#include "kv_attend.cuh"
+
+namespace nbk {
+
+constexpr int WIDE_ROWS = 128, WIDE_KEYS = 128, WIDE_ATT_THREADS = 13 * 32;
+constexpr int WIDE_LOADERS = 128;
+constexpr float SLACK = 6.0f;
+
+// K-major operands without swizzle: 8 rows x 16 bytes make a core matrix of
+// 128 contiguous bytes; `sbo` leads to the next 8 rows, 128 to the next 16 bytes.
+__device__ __forceinline__ uint64_t core_desc(uint32_t addr, uint32_t sbo) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)((sbo >> 4) & 0x3fff) << 32) | (1ull << 46);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+      "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Every wait here is for work of microseconds.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t phase) { return mbar_wait_polls(bar, phase, 1u << 18); }
+
+template <int D>
+struct WideSmem {
+  uint8_t q[2][WIDE_ROWS * D * 2];   // [slot or 0] rows x D
+  uint8_t k[2][WIDE_KEYS * D * 2];   // [stage] keys x D
+  uint8_t v[2][D * WIDE_KEYS * 2];   // [stage] D x keys
+  // per key, four tiles deep (a tile's numbers live from its K's loading until
+  // its P is done; K of tile j is written once S of tile j - 2 is complete)
+  float mul[4][WIDE_KEYS], add[4][WIDE_KEYS], inv[4][WIDE_KEYS];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done;
+  uint32_t tmem;
+  int failed;
+};
+
+// grid (row tiles (or pairs) x sequences, kv heads, parts), block 416
+template <int D, bool BF16, bool E4M3>
+__global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDev a, bool prefix, bool pair, int parts0) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  WideSmem<D>& sm = *reinterpret_cast<WideSmem<D>*>(smem_raw);
+  constexpr uint32_t S_IDESC = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(WIDE_KEYS >> 3) << 17) | ((uint32_t)(WIDE_ROWS >> 4) << 24);
+  constexpr uint32_t O_IDESC = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(WIDE_ROWS >> 4) << 24);
+  constexpr uint32_t ROW_SBO = D / 8 * 128, V_SBO = WIDE_KEYS / 8 * 128;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int h = blockIdx.y, part = blockIdx.z, cover = pair ? 2 * WIDE_ROWS : WIDE_ROWS;
+
+  int token0, tokens, row0, k0, k1, sees0 = 0;
+  const uint32_t* pages;
+  if (prefix) {
+    row0 = blockIdx.x * cover;
+    token0 = 0;
+    tokens = a.b.rows;
+    k0 = part * a.prefix_chunk;
+    k1 = min(a.prefix, k0 + a.prefix_chunk);
+    pages = a.prefix_pages;
+  } else {
+    const int s = blockIdx.x / a.tiles_per_sequence;
+    row0 = (blockIdx.x % a.tiles_per_sequence) * cover;
+    const Span sp = span_of(a.b, s);
+    if (!sp.ok) {
+      if (tid == 0) atomicOr(a.c.error, KV_BAD_SEQUENCE);
+      return;
+    }
+    token0 = sp.first;
+    tokens = sp.n;
+    if (row0 >= tokens * a.group) return;
+    sees0 = sp.len - sp.n;
+    k0 = part * a.tail_chunk;
+    k1 = min(sees0 + min(tokens - 1, (row0 + cover - 1) / a.group) + 1, k0 + a.tail_chunk);
+    pages = a.b.pages + (size_t)s * a.b.page_stride;
+  }
+  const int rows = tokens * a.group;
+  const int tiles = max(0, (k1 - k0 + WIDE_KEYS - 1) / WIDE_KEYS);
+  // events: (key tile, slot) in the order in which the tensor cores take them
+  const int events = pair ? 2 * tiles : tiles;
+
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    sm.failed = 0;
+    for (int i = 0; i < 2; ++i) {
+      bar_init(smem_u32(&sm.k_full[i]), WIDE_LOADERS);
+      bar_init(smem_u32(&sm.v_full[i]), WIDE_LOADERS);
+      bar_init(smem_u32(&sm.k_empty[i]), 1);
+      bar_init(smem_u32(&sm.v_empty[i]), 1);
+      bar_init(smem_u32(&sm.s_full[i]), 1);
+      bar_init(smem_u32(&sm.p_full[i]), WIDE_ROWS);
+    }
+    bar_init(smem_u32(&sm.done), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // the query rows; rows past the end are zeros
+  for (int x = tid; x < cover * (D / 8); x += WIDE_ATT_THREADS) {
+    const int i = x / (D / 8), chunk = x % (D / 8), r = row0 + i;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      const uint16_t* p = static_cast<const uint16_t*>(a.q.data) + (token0 + r / a.group) * a.q.row_stride + (h * a.group + r % a.group) * a.q.head_stride + chunk * 8;
+      if (a.q_vector16) {
+        w = *reinterpret_cast<const uint4*>(p);
+      } else {
+        w.x = p[0] | (uint32_t)p[1] << 16;
+        w.y = p[2] | (uint32_t)p[3] << 16;
+        w.z = p[4] | (uint32_t)p[5] << 16;
+        w.w = p[6] | (uint32_t)p[7] << 16;
+      }
+    }
+    const int t = i & (WIDE_ROWS - 1);
+    *reinterpret_cast<uint4*>(sm.q[i / WIDE_ROWS] + (t / 8) * ROW_SBO + chunk * 128 + (t % 8) * 16) = w;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sm.tmem;
+
+  bool ok = true;
+  if (warp < 8) {
+    // ------------------------------------------------------------- softmax
+    const int slot = warp >> 2;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + slot * 128, o_addr = tmem + lanes + 256 + slot * 128;
+    const int i = (pair ? slot * WIDE_ROWS : 0) + (warp & 3) * 32 + lane, r = row0 + i;
+    const int limit = prefix ? k1 : min(k1, sees0 + min(r, rows - 1) / a.group + 1);
+    // keys below it are seen by every row of the warp
+    const int all_see = prefix ? k1 : min(k1, sees0 + min(r - lane, rows - 1) / a.group + 1);
+    float m = -INFINITY;
+    float2 l2 = make_float2(0.0f, 0.0f);
+    int n = 0;
+    for (int e = slot; e < events && ok; e += 2, ++n) {
+      const int j = pair ? e >> 1 : e, key0 = k0 + j * WIDE_KEYS;
+      ok = __all_sync(FULL, wait(smem_u32(&sm.s_full[slot]), n & 1));
+      if (!ok) break;
+      fence_after();
+      const float* mul = sm.mul[j & 3];
+      const float* add = sm.add[j & 3];
+      const float* inv = sm.inv[j & 3];
+      const bool partial = key0 + WIDE_KEYS > all_see && !prefix;
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < WIDE_KEYS; c += 32) {
+        uint32_t s[32];
+        tmem_load32(s_addr + c, s);
+        tmem_wait_load();
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+          const float4 mu = *reinterpret_cast<const float4*>(mul + c + x), ad = *reinterpret_cast<const float4*>(add + c + x);
+          float2 t0 = fma2(make_float2(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), make_float2(mu.x, mu.y), make_float2(ad.x, ad.y));
+          float2 t1 = fma2(make_float2(__uint_as_float(s[x + 2]), __uint_as_float(s[x + 3])), make_float2(mu.z, mu.w), make_float2(ad.z, ad.w));
+          if (partial) {
+            const int k = key0 + c + x;
+            t0.x = k < limit ? t0.x : -INFINITY;
+            t0.y = k + 1 < limit ? t0.y : -INFINITY;
+            t1.x = k + 2 < limit ? t1.x : -INFINITY;
+            t1.y = k + 3 < limit ? t1.y : -INFINITY;
+          }
+          top = fmaxf(top, fmaxf(fmaxf(t0.x, t0.y), fmaxf(t1.x, t1.y)));
+        }
+      }
+      const float want = __fadd_rn(top, -HEADROOM);
+      const bool grown = want > __fadd_rn(m, SLACK) || m == -INFINITY;
+      if (__any_sync(FULL, grown)) {
+        const float next = grown ? fmaxf(m, want) : m;
+        const float keep = next == m ? 1.0f : ex2(__fadd_rn(m, -next));
+        m = next;
+        l2 = make_float2(__fmul_rn(l2.x, keep), __fmul_rn(l2.y, keep));
+        if (n > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_load32(o_addr + c, o);
+            tmem_wait_load();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__fmul_rn(__uint_as_float(o[x]), keep));
+            tmem_store32(o_addr + c, o);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : -m;
+      const float2 base2 = make_float2(base, base);
+#pragma unroll 1
+      for (int c = 0; c < WIDE_KEYS; c += 32) {
+        uint32_t s[32], p[16];
+        tmem_load32(s_addr + c, s);
+        tmem_wait_load();
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+          const float4 mu = *reinterpret_cast<const float4*>(mul + c + x), ad = *reinterpret_cast<const float4*>(add + c + x);
+          float4 in = *reinterpret_cast<const float4*>(inv + c + x);
+          float2 t0 = fma2(make_float2(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), make_float2(mu.x, mu.y), make_float2(ad.x, ad.y));
+          float2 t1 = fma2(make_float2(__uint_as_float(s[x + 2]), __uint_as_float(s[x + 3])), make_float2(mu.z, mu.w), make_float2(ad.z, ad.w));
+          if (partial) {
+            const int k = key0 + c + x;
+            if (k >= limit) t0.x = -INFINITY, in.x = 0.0f;
+            if (k + 1 >= limit) t0.y = -INFINITY, in.y = 0.0f;
+            if (k + 2 >= limit) t1.x = -INFINITY, in.z = 0.0f;
+            if (k + 3 >= limit) t1.y = -INFINITY, in.w = 0.0f;
+          }
+          t0 = add2(t0, base2);
+          t1 = add2(t1, base2);
+          t0 = make_float2(ex2(t0.x), ex2(t0.y));
+          t1 = make_float2(ex2(t1.x), ex2(t1.y));
+          l2 = fma2(t0, make_float2(in.x, in.y), l2);
+          l2 = fma2(t1, make_float2(in.z, in.w), l2);
+          p[x / 2] = pack_f16(t0.x, t0.y);
+          p[x / 2 + 1] = pack_f16(t1.x, t1.y);
+        }
+        tmem_store16(s_addr + c / 2, p);  // over columns of S that are already read
+      }
+      tmem_wait_store();
+      fence_before();
+      bar_arrive(smem_u32(&sm.p_full[slot]));
+    }
+    if (!ok) sm.failed = 1;
+    if (ok && tiles > 0) ok = __all_sync(FULL, wait(smem_u32(&sm.done), 0));
+    fence_after();
+    // this row's part; a slot without a key tile of its own has sum 0
+    if (ok) {
+      const int index = parts0 + (pair ? part : 2 * part + slot);
+      const size_t at = r < rows ? ((size_t)index * a.b.rows + token0 + r / a.group) * a.heads + h * a.group + r % a.group : 0;
+      if (r < rows) a.part_ml[at] = make_float2(m, __fadd_rn(l2.x, l2.y));
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_load32(o_addr + c, o);
+          tmem_wait_load();
+        } else {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = 0u;
+        }
+        if (r < rows) {
+#pragma unroll
+          for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(a.part_o + at * D + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+        }
+      }
+    }
+  } else if (warp < 12) {
+    // -------------------------------------------------------------- loading
+    const int lw = warp - 8;
+    constexpr int KN = D / 16, VN = D / 32;
+    uint4 kr[KN];
+    uint4 vr[VN][2];
+    float ks = 0.0f, vs = 0.0f;
+    bool page_ok = false;
+    auto fetch = [&](int j) {
+      const int key0 = k0 + j * WIDE_KEYS + lw * 32;  // 32 keys of one page
+      page_ok = false;
+      if (key0 < k1) {
+        const uint32_t page = pages[key0 / KV_PAGE];
+        if (page < a.c.pages) {
+          page_ok = true;
+          const size_t block = (size_t)page * a.c.kv_heads + h;
+          const int in_page = key0 % KV_PAGE;
+          const uint8_t* kp = a.c.k + block * (KV_PAGE * D) + in_page * D;
+          const uint8_t* vp = a.c.v + block * (KV_PAGE * D) + in_page * D;
+          // 8 keys x 4 pieces of 16 codes a load
+#pragma unroll
+          for (int x = 0; x < KN; ++x)
+            kr[x] = *reinterpret_cast<const uint4*>(kp + ((x / (D / 64)) * 8 + (lane & 7)) * D + (x % (D / 64)) * 64 + (lane >> 3) * 16);
+          // two blocks of 16 keys; of each, eight keys of dimension groups 8t + lane % 8
+#pragma unroll
+          for (int x = 0; x < VN; ++x) {
+            const uint8_t* p = vp + (lane >> 4) * 16 * D + x * 512 + (lane & 7) * 64 + ((lane >> 3) & 1) * 32;
+            vr[x][0] = *reinterpret_cast<const uint4*>(p);
+            vr[x][1] = *reinterpret_cast<const uint4*>(p + 16);
+          }
+          ks = a.c.ks[block * KV_PAGE + in_page + lane];
+          vs = a.c.vs[block * KV_PAGE + in_page + lane];
+        } else if (lane == 0) {
+          atomicOr(a.c.error, KV_BAD_PAGE);
+        }
+      }
+      if (!page_ok) {
+#pragma unroll
+        for (int x = 0; x < KN; ++x) kr[x] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < VN; ++x) vr[x][0] = vr[x][1] = make_uint4(0, 0, 0, 0);
+      }
+    };
+    if (tiles > 0) fetch(0);
+    for (int j = 0; j < tiles && ok; ++j) {
+      const int stage = j & 1;
+      if (j >= 2) ok = wait(smem_u32(&sm.k_empty[stage]), ((j >> 1) - 1) & 1);
+      if (!ok) break;
+      {
+        const int key = lw * 32 + lane;
+        const bool seen = page_ok && k0 + j * WIDE_KEYS + key < k1;
+        sm.mul[j & 3][key] = seen ? __fmul_rn(ks, a.scale) : 0.0f;
+        sm.add[j & 3][key] = seen ? lg2(vs) : -INFINITY;
+        sm.inv[j & 3][key] = seen ? __frcp_rn(vs) : 0.0f;
+      }
+#pragma unroll
+      for (int x = 0; x < KN; ++x) {
+        const uint32_t w[4] = {kr[x].x, kr[x].y, kr[x].z, kr[x].w};
+        uint8_t* dst = sm.k[stage] + (lw * 4 + x / (D / 64)) * ROW_SBO + ((x % (D / 64)) * 8 + (lane >> 3) * 2) * 128 + (lane & 7) * 16;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint2 lo = widen<E4M3, BF16>(w[2 * y]), hi = widen<E4M3, BF16>(w[2 * y + 1]);
+          *reinterpret_cast<uint4*>(dst + y * 128) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(smem_u32(&sm.k_full[stage]));
+      if (j >= 2) ok = wait(smem_u32(&sm.v_empty[stage]), ((j >> 1) - 1) & 1);
+      if (!ok) break;
+#pragma unroll
+      for (int x = 0; x < VN; ++x) {
+        const uint32_t w0[4] = {vr[x][0].x, vr[x][0].y, vr[x][0].z, vr[x][0].w}, w1[4] = {vr[x][1].x, vr[x][1].y, vr[x][1].z, vr[x][1].w};
+        uint8_t* dst = sm.v[stage] + (lw * 4 + (lane >> 4) * 2 + ((lane >> 3) & 1)) * 128 + (lane & 7) * 16;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint2 lo = widen<E4M3, false>(w0[t]), hi = widen<E4M3, false>(w1[t]);
+          *reinterpret_cast<uint4*>(dst + (x * 4 + t) * V_SBO) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(smem_u32(&sm.v_full[stage]));
+      if (j + 1 < tiles) fetch(j + 1);
+    }
+    if (!ok) sm.failed = 1;
+  } else {
+    if (lane == 0 && events > 0) {
+      // ------------------------------------------------ the matrix instructions
+      const uint32_t q_addr = smem_u32(sm.q[0]);
+      auto scores = [&](int e) {
+        const int slot = e & 1, j = pair ? e >> 1 : e, stage = j & 1;
+        if (!pair || slot == 0) {
+          ok = ok && wait(smem_u32(&sm.k_full[stage]), (j >> 1) & 1);
+          fence_after();
+        }
+        if (!ok) return;
+        const uint32_t qa = q_addr + (pair ? slot * WIDE_ROWS * D * 2 : 0), ka = smem_u32(sm.k[stage]);
+  #pragma unroll
+        for (int x = 0; x < D / 16; ++x)
+          mma_ss(tmem + slot * 128, core_desc(qa + x * 256, ROW_SBO), core_desc(ka + x * 256, ROW_SBO), S_IDESC, x > 0);
+        mma_commit(smem_u32(&sm.s_full[slot]));
+        if (!pair || slot == 1) mma_commit(smem_u32(&sm.k_empty[stage]));
+      };
+      scores(0);
+      if (events > 1) scores(1);
+      for (int e = 0; e < events && ok; ++e) {
+        const int slot = e & 1, j = pair ? e >> 1 : e, stage = j & 1;
+        ok = wait(smem_u32(&sm.p_full[slot]), (e >> 1) & 1);
+        if (ok && (!pair || slot == 0)) ok = wait(smem_u32(&sm.v_full[stage]), (j >> 1) & 1);
+        if (!ok) break;
+        fence_after();
+        const uint32_t va = smem_u32(sm.v[stage]);
+  #pragma unroll
+        for (int x = 0; x < WIDE_KEYS / 16; ++x)
+          mma_ts(tmem + 256 + slot * 128, tmem + slot * 128 + x * 8, core_desc(va + x * 256, V_SBO), O_IDESC, e >= 2 || x > 0);
+        if (!pair || slot == 1) mma_commit(smem_u32(&sm.v_empty[stage]));
+        if (e + 2 < events) scores(e + 2);
+      }
+      mma_commit(smem_u32(&sm.done));
+      if (!ok) {
+        sm.failed = 1;
+        wait(smem_u32(&sm.done), 0);  // what was issued ends before the TMEM is freed
+      }
+    }
+    __syncwarp();
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (lane == 0 && *static_cast<volatile int*>(&sm.failed)) atomicOr(a.c.error, KV_WAIT_FAILED);
+  }
+}
+
+template <int D, bool BF16, bool E4M3>
+static cudaError_t wide_launch(const AttendDev& a, bool prefix, int tiles, int chunks, cudaStream_t st) {
+  static_assert(sizeof(WideSmem<D>) <= 227 * 1024, "fits an SM's shared memory");
+  auto kernel = k_kv_attend_wide<D, BF16, E4M3>;
+  // an attribute of the current device's context; setting it is idempotent and cheap beside the launch
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(WideSmem<D>));
+  if (e != cudaSuccess) return e;
+  const bool pair = prefix ? a.prefix_pair : a.tail_pair;
+  kernel<<<dim3((unsigned)tiles, (unsigned)a.c.kv_heads, (unsigned)chunks), WIDE_ATT_THREADS, sizeof(WideSmem<D>), st>>>(a, prefix, pair,
+                                                                                                               prefix ? 0 : a.prefix_parts);
+  return cudaGetLastError();
+}
+
+cudaError_t attend_wide(const AttendDev& a, bool prefix, int tiles, int chunks, cudaStream_t st) {
+  const bool bf16 = a.q.dtype == DTYPE_BF16;
+  if (a.c.dim == 64) {
+    if (bf16) return a.c.e4m3 ? wide_launch<64, true, true>(a, prefix, tiles, chunks, st) : wide_launch<64, true, false>(a, prefix, tiles, chunks, st);
+    return a.c.e4m3 ? wide_launch<64, false, true>(a, prefix, tiles, chunks, st) : wide_launch<64, false, false>(a, prefix, tiles, chunks, st);
+  }
+  if (bf16) return a.c.e4m3 ? wide_launch<128, true, true>(a, prefix, tiles, chunks, st) : wide_launch<128, true, false>(a, prefix, tiles, chunks, st);
+  return a.c.e4m3 ? wide_launch<128, false, true>(a, prefix, tiles, chunks, st) : wide_launch<128, false, false>(a, prefix, tiles, chunks, st);
+}
+
+}  // namespace nbk
