@@ -17,6 +17,7 @@
 #include <cooperative_groups.h>
 
 #include <cfloat>
+#include <type_traits>
 
 #include "serving.cuh"
 
@@ -24,7 +25,7 @@ namespace nbk {
 
 namespace cg = cooperative_groups;
 
-constexpr int VERIFY_THREADS = 512, VERIFY_WARPS = VERIFY_THREADS / 32, VERIFY_MAX_CLUSTER = 8, VERIFY_MAX_ROWS = 8;
+constexpr int VERIFY_MAX_CLUSTER = 8, VERIFY_MAX_ROWS = 8, VERIFY_MAX_WARPS = 16;
 constexpr uint32_t NO_TOKEN = 0xffffffffu;
 
 // A logit as the formulas take it: NaN counts as -inf (fmaxf drops it), +inf
@@ -46,6 +47,8 @@ struct LogitRow {
   // the same for every row of a launch: pieces that any alignment needs
   __device__ __forceinline__ static int pieces(int v) { return v / N + 2; }
   __device__ __forceinline__ int start(int piece) const { return head + (piece - 1) * N; }
+  // pieces [1, whole_end()) lie whole within the row
+  __device__ __forceinline__ int whole_end() const { return (vocab - head) / N + 1; }
   __device__ __forceinline__ bool whole(int piece) const { return start(piece) >= 0 && start(piece) + N <= vocab; }
   __device__ __forceinline__ bool permits(int id) const { return !allowed || (allowed[id >> 5] >> (id & 31) & 1); }
   // which of a piece's ids exist and are allowed
@@ -83,10 +86,20 @@ struct LogitRow {
     return w;
   }
   __device__ __forceinline__ static void widen_piece(const uint4& w, float (&x)[N]) {
-    T t[N];
-    memcpy(t, &w, 16);
+    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = to_f32(t[i]);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (N == 4) {
+        x[i] = __uint_as_float(word[i]);
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        x[2 * i] = __uint_as_float(word[i] << 16);
+        x[2 * i + 1] = __uint_as_float(word[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&word[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
   }
 };
 
@@ -96,36 +109,192 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// 2^(y / 64) for y <= 0 in f64: y = k + f, k whole, |f| <= 1/2; the table holds
-// 2^(j / 64), and e^r with r = f ln2 / 64 (|r| <= 0.0055) is its Taylor
-// polynomial of degree 5 (remainder below 1e-16).
-__device__ __forceinline__ double exp2_64th(double y, const double* table) {
-  if (y < -64.0 * 1000.0) return 0.0;
+// 2^(y / 128) for -128000 <= y <= 0 in f64: y = k + f, k whole, |f| <= 1/2; the
+// table holds 2^(j / 128), sixteen times over so that no two lanes of a half
+// warp meet in a bank, and 2^(f / 128) = e^r with r = f ln2 / 128 (|r| <=
+// 0.0028) is its Taylor polynomial of degree 3, within 3e-12 relative. The
+// power of two goes into the table's value: 2^(y / 128) = e · t. Entry j's high
+// word is kept less j 2^13, so that adding k 2^13 leaves k / 128 in the exponent.
+constexpr int EXP_ENTRIES = 128, EXP_COPIES = 16;
+struct Exp2Table {
+  double entry[EXP_ENTRIES];
+};
+// 2^(j / 128) by the exponential's series, and its high word less j 2^13. The
+// high word is at least 0x3ff00000 - 127 · 2^13 > 0 and the sum below restores
+// it, so the entry is taken apart only as bits.
+constexpr Exp2Table exp2_table() {
+  Exp2Table t{};
+  for (int j = 0; j < EXP_ENTRIES; ++j) {
+    const double r = j * (0.693147180559945309417 / EXP_ENTRIES);
+    double sum = 1.0;
+    for (int n = 24; n > 0; --n) sum = 1.0 + sum * r / n;
+    // sum = 1 + m 2^-52 with a whole m; taking j 2^13 from the high word takes
+    // j 2^-7 from the mantissa, and one from the exponent where that borrows
+    const double less = j / 128.0, mantissa = sum - 1.0;
+    t.entry[j] = mantissa >= less ? 1.0 + (mantissa - less) : 0.5 * (1.0 + (mantissa - less + 1.0));
+  }
+  return t;
+}
+__device__ const Exp2Table g_exp2_table = exp2_table();
+
+struct Exp2Parts {
+  double e, t;
+};
+__device__ __forceinline__ Exp2Parts exp2_128th(double y, const double* table) {
+  constexpr double C = 0.693147180559945309417 / EXP_ENTRIES, C2 = C * C / 2.0, C3 = C2 * C / 3.0;
   const double shifted = y + 6755399441055744.0;  // 1.5 · 2^52: rounds to a whole number, held in the low bits
   const int k = __double2loint(shifted);
-  const double r = (y - (shifted - 6755399441055744.0)) * (0.693147180559945309417 / 64.0);
-  double e = __fma_rn(r, 1.0 / 120.0, 1.0 / 24.0);
-  e = __fma_rn(e, r, 1.0 / 6.0);
-  e = __fma_rn(e, r, 0.5);
-  e = __fma_rn(e, r, 1.0);
-  e = __fma_rn(e, r, 1.0);
-  e *= table[k & 63];
-  return __hiloint2double(__double2hiint(e) + ((k >> 6) << 20), __double2loint(e));  // e in [0.99, 2), k / 64 >= -1000
+  const double f = y - (shifted - 6755399441055744.0);
+  Exp2Parts x;
+  x.e = __fma_rn(f, C3, C2);
+  x.e = __fma_rn(x.e, f, C);
+  x.e = __fma_rn(x.e, f, 1.0);
+  const double t = *reinterpret_cast<const double*>(reinterpret_cast<const char*>(table) + ((k << 7) & ((EXP_ENTRIES - 1) << 7)));
+  x.t = __hiloint2double(__double2hiint(t) + (k << (20 - 7)), __double2loint(t));  // k / 128 >= -1000
+  return x;
+}
+
+// A thread's part of a row: the maximum (greedy: and its lowest id) and the sum
+// of e^((x - m) / T). `base` is fl(m step) and `shift` 2^(base - m step): a
+// weight is 2^(x step - base), one multiply-add and one exponential, and the
+// sum of a batch comes to m by one product.
+template <bool GREEDY>
+struct RowStats {
+  float m = -INFINITY, sum = 0.0f, base = 0.0f, shift = 1.0f;
+  int where = INT_MAX;
+  bool any = false;  // an id is allowed
+};
+constexpr float BASE_MOST = 32768.0f;  // beyond it, base is too coarse for the product
+
+// The pieces c, c + stride, .. below `end`, A of them at once so that their
+// loads overlap and the maximum is looked at once for all. CLEAN: they are
+// whole and no id is masked.
+template <typename T, bool GREEDY, int A, bool CLEAN>
+__device__ __forceinline__ void take_pieces(const LogitRow<T>& row, int c, int stride, int end, float step, RowStats<GREEDY>& st) {
+  constexpr int N = LogitRow<T>::N;
+  constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+  uint4 w[A];
+  uint32_t bits[A];
+#pragma unroll
+  for (int a = 0; a < A; ++a) {
+    const int k = c + a * stride;
+    w[a] = make_uint4(NONE, NONE, NONE, NONE);
+    bits[a] = 0;
+    if (CLEAN) {
+      if (k < end) w[a] = *reinterpret_cast<const uint4*>(row.p + row.start(k));
+    } else {
+      if (k < end) w[a] = row.raw(k), bits[a] = row.live(k);
+    }
+  }
+  float x[A * N];
+#pragma unroll
+  for (int a = 0; a < A; ++a) {
+    float t[N];
+    LogitRow<T>::widen_piece(w[a], t);
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[a * N + e] = CLEAN ? t[e] : bits[a] >> e & 1 ? tame(t[e]) : -INFINITY;
+    st.any = st.any || CLEAN || bits[a];
+  }
+  float high = x[0];
+#pragma unroll
+  for (int e = 1; e < A * N; ++e) high = fmaxf(high, x[e]);  // drops NaN
+  if (high > st.m) {
+    if (CLEAN && high > FLT_MAX) {  // +inf among them
+#pragma unroll
+      for (int e = 0; e < A * N; ++e) x[e] = tame(x[e]);
+      high = FLT_MAX;
+    }
+    if (!GREEDY) {
+      st.sum = __fmul_rn(st.sum, exp2_fast(__fmul_rn(__fadd_rn(st.m, -high), step)));
+      st.base = __fmul_rn(high, step);
+      st.shift = exp2_fast(-__fmaf_rn(high, step, -st.base));
+    } else if (high > st.m) {
+#pragma unroll
+      for (int e = A * N - 1; e >= 0; --e)
+        if (x[e] == high) st.where = row.start(c + e / N * stride) + e % N;
+    }
+    st.m = high;
+  }
+  if (!GREEDY && st.m != -INFINITY) {
+    float add = 0.0f;
+    const float base = st.base;
+    if (fabsf(base) <= BASE_MOST) {
+#pragma unroll
+      for (int e = 0; e < A * N; ++e) add = __fadd_rn(add, exp2_fast(__fmaf_rn(x[e], step, -base)));
+      add = __fmul_rn(add, st.shift);
+    }
+    if (!(fabsf(base) <= BASE_MOST) || add != add) {  // very large logits, or a NaN among them
+      add = 0.0f;
+#pragma unroll
+      for (int e = 0; e < A * N; ++e) add = __fadd_rn(add, exp2_fast(__fmul_rn(__fadd_rn(tame(x[e]), -st.m), step)));
+    }
+    st.sum = __fadd_rn(st.sum, add);
+  }
+}
+
+constexpr int DRAFTS = 64;  // whose numbers are held at once, a multiple of the rows of a round
+constexpr int DRAW_GROUPS = 4;
+constexpr double FLOOR = -124000.0;                    // of exp2_128th's argument: 2^-968
+constexpr double GHOST = 1e-289, GHOSTS = 1e-280;  // a share, a sum of shares, that counts as none
+
+// A piece as it lies in memory, its live ids, and the draft's probabilities.
+template <int N>
+struct Piece {
+  uint4 w;
+  uint32_t bits;
+  float q[N];
+};
+struct Draw {
+  const double* table;
+  float lowest, top;
+  double scale;  // (x - top) · scale is the exponential's argument
+  double lift;   // 128 log2 of 1 / the sum of the weights, once that is known
+  double offset; // lift - top · scale, where that is small enough to be exact
+};
+
+// A piece's weights, or (LESS) what the probabilities have above q; without
+// branches, so that the chains of several elements overlap. ALL: every id is
+// live, and the logits are of a size (2^30 of the exponential's steps) whose
+// product with the scale is off by 2^-23 of a step at most, the same for all.
+template <typename T, bool LESS, bool ALL>
+__device__ __forceinline__ void piece_shares(const Piece<LogitRow<T>::N>& p, const Draw& d, double (&x)[LogitRow<T>::N]) {
+  constexpr int N = LogitRow<T>::N;
+  float f[N];
+  LogitRow<T>::widen_piece(p.w, f);
+  const double top = d.top;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    float t = fmaxf(f[e], d.lowest);
+    if (!ALL) t = fminf(t, d.top);
+    double y = ALL ? __fma_rn((double)t, d.scale, d.offset) : __fma_rn((double)t - top, d.scale, d.lift);
+    if (!ALL) y = (p.bits >> e & 1) && f[e] > -INFINITY ? y : FLOOR;
+    const Exp2Parts w = exp2_128th(y, d.table);
+    if (LESS) {
+      const double r = __fma_rn(w.e, w.t, -(double)p.q[e]);
+      x[e] = __double2hiint(r) < 0 ? 0.0 : r;  // a NaN stays
+    } else {
+      x[e] = w.e * w.t;
+    }
+  }
 }
 
 struct VerifyShared {
-  float top[2][VERIFY_MAX_CLUSTER * VERIFY_WARPS];  // every warp's results of a round, in turn
-  float sum[2][VERIFY_MAX_CLUSTER * VERIFY_WARPS];
-  int at[2][VERIFY_MAX_CLUSTER * VERIFY_WARPS];  // greedy: the maximum's lowest id; else 0 when an id is allowed, INT_MAX when none
-  double draw[2][VERIFY_MAX_CLUSTER * VERIFY_WARPS];
+  float top[2][VERIFY_MAX_CLUSTER * VERIFY_MAX_WARPS];  // every warp's results of a round, in turn
+  float sum[2][VERIFY_MAX_CLUSTER * VERIFY_MAX_WARPS];
+  int at[2][VERIFY_MAX_CLUSTER * VERIFY_MAX_WARPS];  // greedy: the maximum's lowest id; else 0 when an id is allowed, INT_MAX when none
+  double draw[2][VERIFY_MAX_CLUSTER * VERIFY_MAX_WARPS];
+  double group[2][VERIFY_MAX_WARPS][DRAW_GROUPS];  // this CTA's: sums of a warp's run, piece by piece
   float row_top[VERIFY_MAX_ROWS];
   int row_at[VERIFY_MAX_ROWS];
+  uint32_t draft[DRAFTS];
+  float draft_logit[DRAFTS], draft_q[DRAFTS], uniform[DRAFTS];
+  int draft_allowed[DRAFTS];
   bool row_accept[VERIFY_MAX_ROWS];
-  double table[64];
+  double table[EXP_ENTRIES * EXP_COPIES];
 };
 
-template <typename T, bool GREEDY>
-__global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int at_once) {
+template <typename T, bool GREEDY, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_verify(VerifyDev v, int at_once) {
   constexpr int N = LogitRow<T>::N;
   __shared__ VerifyShared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -136,81 +305,74 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int a
   const int drafts = v.draft_counts ? max(0, min(v.drafts, v.draft_counts[s])) : v.drafts;
   const double inverse = GREEDY ? 1.0 : 1.0 / (double)v.temperature;
   const float step = (float)(inverse * 1.4426950408889634);
-  if (!GREEDY && tid < 64) sh.table[tid] = exp2((double)tid / 64.0);
+  if (!GREEDY)
+    for (int i = tid; i < EXP_ENTRIES * EXP_COPIES; i += (WARPS * 32)) sh.table[i] = g_exp2_table.entry[i / EXP_COPIES];
   auto row_of = [&](int i, bool unmasked) {
     return LogitRow<T>(static_cast<const T*>(v.logits) + ((long long)s * (v.drafts + 1) + i) * v.row_stride,
                        v.mask && !unmasked ? v.mask + ((size_t)s * (v.drafts + 1) + i) * words : nullptr, v.vocab);
   };
 
-  const int row_warps = VERIFY_WARPS / at_once;
+  const int row_warps = WARPS / at_once;
   int turn = 0, kept = 0, best = 0;
   float top = -INFINITY;
   uint32_t unmasked = 0;  // rows of the round whose mask allows nothing
-  bool stop = false;
+  bool stop = false, redo = false;
   for (int i0 = 0; !stop;) {
     const int mine = warp / row_warps;
-    {
-      const int i = i0 + mine;
-      float m = -INFINITY, sum = 0.0f;
-      int where = INT_MAX;
-      bool any = false;
-      if (i <= drafts) {
-        const LogitRow<T> row = row_of(i, unmasked >> mine & 1);
-        constexpr int AHEAD = 4;
-        const int stride = row_warps * 32;
-        for (int c0 = lo + (warp % row_warps) * 32 + lane; c0 < hi; c0 += AHEAD * stride) {
-          uint4 w[AHEAD];
-#pragma unroll
-          for (int a = 0; a < AHEAD; ++a)
-            if (c0 + a * stride < hi) w[a] = row.raw(c0 + a * stride);
-#pragma unroll
-          for (int a = 0; a < AHEAD; ++a) {
-            const int c = c0 + a * stride;
-            if (c >= hi) break;
-            float x[N];
-            LogitRow<T>::widen_piece(w[a], x);
-            const bool plain = !row.allowed && row.whole(c);
-            const uint32_t bits = plain ? (1u << N) - 1 : row.live(c);
-            any = any || bits;
-            float high = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-              x[e] = plain || (bits >> e & 1) ? tame(x[e]) : -INFINITY;
-              high = fmaxf(high, x[e]);
-            }
-            if (high > m) {
-              if (!GREEDY) sum = __fmul_rn(sum, exp2_fast(__fmul_rn(__fadd_rn(m, -high), step)));
-              m = high;
-              if (GREEDY) {
-#pragma unroll
-                for (int e = N - 1; e >= 0; --e)
-                  if (x[e] == high) where = row.start(c) + e;
-              }
-            }
-            if (!GREEDY && m != -INFINITY) {
-              float add = 0.0f;
-#pragma unroll
-              for (int e = 0; e < N; ++e) add = __fadd_rn(add, exp2_fast(__fmul_rn(__fadd_rn(x[e], -m), step)));
-              sum = __fadd_rn(sum, add);
-            }
-          }
+    // what the decisions need of the drafts, DRAFTS rows ahead: two dependent
+    // loads from far, taken once by the last warps
+    if (i0 % DRAFTS == 0 && !redo && tid >= WARPS * 32 - DRAFTS) {
+      const int k = tid - (WARPS * 32 - DRAFTS), i = i0 + k;
+      if (i < drafts) {
+        const size_t at = (size_t)s * v.drafts + i;
+        const uint32_t d = v.draft_tokens[at];
+        sh.draft[k] = d;
+        if (!GREEDY) {
+          sh.uniform[k] = v.accept[at];
+          const bool known = d < (uint32_t)v.vocab;
+          const LogitRow<T> row = row_of(i, true);
+          sh.draft_logit[k] = known ? tame(to_f32(row.p[d])) : -INFINITY;
+          sh.draft_q[k] = known && v.q ? v.q[at * v.vocab + d] : 1.0f;
+          sh.draft_allowed[k] = known && v.mask ? v.mask[((size_t)s * (v.drafts + 1) + i) * words + (d >> 5)] >> (d & 31) & 1 : 1;
         }
       }
+    }
+    {
+      const int i = i0 + mine;
+      RowStats<GREEDY> st;
+      if (i <= drafts) {
+        const LogitRow<T> row = row_of(i, unmasked >> mine & 1);
+        const int stride = row_warps * 32;
+        int c = lo + (warp % row_warps) * 32 + lane;
+        if (!row.allowed) {
+          if (c == 0) take_pieces<T, GREEDY, 1, false>(row, 0, stride, hi, step, st), c += stride;
+          constexpr int A = N == 8 ? 4 : 8;
+          const int whole = min(hi, row.whole_end());
+          for (; c < whole; c += A * stride) take_pieces<T, GREEDY, A, true>(row, c, stride, whole, step, st);
+          // what is left are the row's last pieces, short or empty
+          if (whole < hi && tid % (row_warps * 32) == 0)
+            for (int k = max(lo, whole); k < hi; ++k) take_pieces<T, GREEDY, 1, false>(row, k, 1, hi, step, st);
+        } else {
+          for (; c < hi; c += 4 * stride) take_pieces<T, GREEDY, 4, false>(row, c, stride, hi, step, st);
+        }
+      }
+      const float m = st.m;
+      float sum = st.sum;
       float wm = m;
 #pragma unroll
       for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(FULL, wm, o));
       int wat;
       if (GREEDY) {
         // a row of -inf alone has ids, but none to choose
-        wat = __reduce_min_sync(FULL, m == wm ? (where == INT_MAX && any ? INT_MAX - 1 : where) : INT_MAX);
+        wat = __reduce_min_sync(FULL, m == wm ? (st.where == INT_MAX && st.any ? INT_MAX - 1 : st.where) : INT_MAX);
       } else {
-        wat = __any_sync(FULL, any) ? 0 : INT_MAX;
+        wat = __any_sync(FULL, st.any) ? 0 : INT_MAX;
         sum = m == -INFINITY ? 0.0f : __fmul_rn(sum, exp2_fast(__fmul_rn(__fadd_rn(m, -wm), step)));
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(FULL, sum, o));
       }
       if (lane < ranks) {
-        const int k = rank * VERIFY_WARPS + warp;
+        const int k = rank * WARPS + warp;
         *cluster.map_shared_rank(&sh.top[turn][k], lane) = wm;
         *cluster.map_shared_rank(&sh.at[turn][k], lane) = wat;
         if (!GREEDY) *cluster.map_shared_rank(&sh.sum[turn][k], lane) = sum;
@@ -220,7 +382,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int a
     // warp r joins the round's row r and decides on its draft
     if (warp < at_once && i0 + warp <= drafts) {
       const int i = i0 + warp, count = ranks * row_warps;
-      auto entry = [&](int k) { return (k / row_warps) * VERIFY_WARPS + warp * row_warps + k % row_warps; };
+      auto entry = [&](int k) { return (k / row_warps) * WARPS + warp * row_warps + k % row_warps; };
       float m = -INFINITY;
       for (int k = lane; k < count; k += 32) m = fmaxf(m, sh.top[turn][entry(k)]);
 #pragma unroll
@@ -235,18 +397,15 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int a
       at = __reduce_min_sync(FULL, at);
       bool accept = false;
       if (i < drafts) {
-        const uint32_t d = v.draft_tokens[(size_t)s * v.drafts + i];
         if (GREEDY) {
-          accept = d == (uint32_t)at;
+          accept = sh.draft[i % DRAFTS] == (uint32_t)at;
         } else {
 #pragma unroll
           for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
-          const LogitRow<T> row = row_of(i, unmasked >> warp & 1);
-          if (d < (uint32_t)v.vocab && m != -INFINITY && row.permits((int)d)) {
-            const double p = exp(((double)tame(to_f32(row.p[d])) - (double)m) * inverse) / total;
-            const double q = v.q ? (double)v.q[((size_t)s * v.drafts + i) * v.vocab + d] : 1.0;
-            accept = (double)v.accept[(size_t)s * v.drafts + i] * q < p;
-          }
+          const int k = i % DRAFTS;
+          const float x = sh.draft_logit[k];
+          if (x != -INFINITY && (sh.draft_allowed[k] || (unmasked >> warp & 1)))
+            accept = (double)sh.uniform[k] * (double)sh.draft_q[k] * total < exp(((double)x - (double)m) * inverse);
         }
       }
       if (lane == 0) {
@@ -269,6 +428,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int a
     }
     // the other set next: a slower CTA may still read this one
     turn ^= 1;
+    redo = again != 0;
     if (again) {
       kept = i0;  // the round once more, with that row unmasked
       unmasked |= again;
@@ -282,7 +442,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int a
 
   uint32_t* out = v.tokens + (size_t)s * (v.drafts + 1);
   if (rank == 0) {
-    for (int i = tid; i <= v.drafts; i += VERIFY_THREADS) {
+    for (int i = tid; i <= v.drafts; i += (WARPS * 32)) {
       if (i < kept) out[i] = v.draft_tokens[(size_t)s * v.drafts + i];
       if (i > kept || (i == kept && top == -INFINITY)) out[i] = NO_TOKEN;
       if (GREEDY && i == kept && top != -INFINITY) out[i] = (uint32_t)best;
@@ -298,7 +458,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int a
   // warps' sums go to every CTA, which finds the same warp; that warp finds
   // the id.
   const LogitRow<T> row = row_of(kept, unmasked);
-  const int run = (hi - lo + VERIFY_WARPS - 1) / VERIFY_WARPS;
+  const int run = (hi - lo + WARPS - 1) / WARPS;
   const int from = min(hi, lo + warp * run), to = min(hi, from + run);
   const float* q = nullptr;
   int certain = -1;  // a draft without probabilities: q is 1 there
@@ -309,73 +469,133 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int a
       certain = (int)min(v.draft_tokens[(size_t)s * v.drafts + kept], (uint32_t)INT_MAX);
   }
   bool residual = kept < drafts;
-  const double scale = inverse * (64.0 * 1.44269504088896340736);
-  double over = 1.0;  // 1 / sum of the weights
-  // a piece's weights, or with `less` what they have above q
-  auto piece_shares = [&](int c, bool less, double (&x)[N]) {
-    const uint4 w = row.raw(c);
-    const uint32_t bits = row.live(c);
+  // No weight is below e^-670 of the largest: -inf, NaN and what is not allowed
+  // come to that too, and shares up to GHOST count as none. Where the logits are
+  // so large that their neighbours are further apart, only the largest counts.
+  const float lowest = fmaxf(fminf(__fadd_ru(top, -__fmul_rd(670.0f, v.temperature)), __fadd_rd(top, -1e-45f)), -FLT_MAX);
+  Draw draw;
+  draw.table = sh.table + (lane & (EXP_COPIES - 1));
+  draw.lowest = lowest;
+  draw.top = top;
+  draw.lift = 0.0;
+  draw.scale = fmin(inverse * (EXP_ENTRIES * 1.44269504088896340736), -FLOOR / ((double)top - (double)lowest));
+  draw.offset = -(double)top * draw.scale;
+  // also where the largest logit is the lowest f32 or the largest: -inf, or +inf, needs a look of its own
+  const bool edge = fabs(draw.offset) > 0x1p30;
+  const int whole_end = row.allowed || edge ? 0 : row.whole_end();  // pieces [1, whole_end) are whole and all allowed
+  auto fetch = [&](int c, bool less, Piece<N>& x) {
     const int e0 = row.start(c);
-    float f[N];
-    LogitRow<T>::widen_piece(w, f);
+    if (c > 0 && c < whole_end) {
+      x.w = *reinterpret_cast<const uint4*>(row.p + e0);
+      x.bits = (1u << N) - 1;
+    } else {
+      x.w = row.raw(c);
+      x.bits = row.live(c);
+    }
+    if (less) {
+      if (q && e0 >= 4 && e0 + N + 4 <= v.vocab) {
+        // 16-byte loads around the piece; where it starts within them is the same for all pieces of the row
+        const float* at = q + e0;
+        const int shift = (int)(reinterpret_cast<uintptr_t>(at) / 4 % 4);
+        const float4* wide = reinterpret_cast<const float4*>(at - shift);
+        float f[N + 4];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      double y = 0.0;
-      if (bits >> e & 1) {
-        const float t = tame(f[e]);
-        if (t != -INFINITY) y = exp2_64th(((double)t - (double)top) * scale, sh.table);
-        if (less) {
-          const double minus = q ? (double)q[e0 + e] : e0 + e == certain ? 1.0 : 0.0;
-          y = fmax(__fma_rn(y, over, -minus), 0.0);
+        for (int k = 0; k < N / 4; ++k) *reinterpret_cast<float4*>(f + 4 * k) = wide[k];
+        if (shift) *reinterpret_cast<float4*>(f + N) = wide[N / 4];
+        if (shift == 0) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) x.q[e] = f[e];
+        } else if (shift == 1) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) x.q[e] = f[e + 1];
+        } else if (shift == 2) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) x.q[e] = f[e + 2];
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) x.q[e] = f[e + 3];
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x.q[e] = q && e0 + e >= 0 && e0 + e < v.vocab ? q[e0 + e] : e0 + e == certain ? 1.0f : 0.0f;
       }
-      x[e] = y;
     }
   };
-  auto all_sums = [&](bool less) {  // sh.draw[turn] = every warp's sum
-    double mine = 0.0;
-    for (int c = from + lane; c < to; c += 32) {
-      double x[N];
-      piece_shares(c, less, x);
-#pragma unroll
-      for (int e = 0; e < N; ++e) mine += x[e];
+  const auto shares = [&](const Piece<N>& p, bool less, double (&x)[N]) {
+    if (p.bits == (1u << N) - 1 && !edge) {
+      if (less)
+        piece_shares<T, true, true>(p, draw, x);
+      else
+        piece_shares<T, false, true>(p, draw, x);
+    } else {
+      if (less)
+        piece_shares<T, true, false>(p, draw, x);
+      else
+        piece_shares<T, false, false>(p, draw, x);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(FULL, mine, o);
-    if (lane < ranks) *cluster.map_shared_rank(&sh.draw[turn][rank * VERIFY_WARPS + warp], lane) = mine;
-    cluster.sync();
   };
-  const int count = ranks * VERIFY_WARPS;
-  auto sum_up = [&] {
-    double x = 0.0;
-    for (int k = lane; k < count; k += 32) x += sh.draw[turn][k];
+  // a run is gone through 32 pieces a step, its steps in DRAW_GROUPS groups
+  const int steps = (run + 31) / 32, group = (steps + DRAW_GROUPS - 1) / DRAW_GROUPS * 32;
+  auto warp_sum = [](double x) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(FULL, x, o);
     return x;
   };
+  auto all_sums = [&](bool less) {  // sh.group[turn] and, in every CTA, sh.draw[turn] = every warp's sum
+    double whole = 0.0;
+    Piece<N> next;
+    if (from + lane < to) fetch(from + lane, less, next);
+    for (int g = 0, g0 = from; g < DRAW_GROUPS && g0 < to; ++g, g0 += group) {
+      double mine = 0.0;
+      for (int c = g0 + lane; c < min(to, g0 + group); c += 32) {
+        const Piece<N> now = next;
+        if (c + 32 < to) fetch(c + 32, less, next);
+        double x[N];
+        shares(now, less, x);
+#pragma unroll
+        for (int e = 0; e < N; e += 2) mine += x[e] + x[e + 1];
+      }
+      mine = warp_sum(mine);
+      if (lane == 0) sh.group[turn][warp][g] = mine;
+      whole += mine;
+    }
+    __syncwarp();
+    if (lane < ranks) *cluster.map_shared_rank(&sh.draw[turn][rank * WARPS + warp], lane) = whole;
+    cluster.sync();
+  };
+  const int count = ranks * WARPS;
+  auto sum_up = [&] {
+    double x = 0.0;
+    for (int k = lane; k < count; k += 32) x += sh.draw[turn][k];
+    return warp_sum(x);
+  };
   all_sums(false);
   double whole = sum_up();
   if (residual) {
-    over = 1.0 / whole;
+    draw.lift = -(double)EXP_ENTRIES * log2(whole);
+    draw.offset += draw.lift;
     const int first = turn;
     turn ^= 1;
     all_sums(true);
     const double left = sum_up();
-    if (left > 0.0) {
+    if (left > GHOSTS) {
       whole = left;
     } else {
       residual = false;  // p nowhere exceeds q: from p
+      draw.offset -= draw.lift;
+      draw.lift = 0.0;
       turn = first;
     }
   }
-  const double goal = (double)v.sample[s] * whole;
+  double goal = (double)v.sample[s] * whole;
+  goal = goal < GHOSTS ? GHOSTS : goal;  // what counts as none is never drawn; a NaN stays
   // the first warp whose running sum passes the goal; 4 neighbouring sums a lane
   double own[4], upto = 0.0;
   int last = -1;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     own[k] = lane * 4 + k < count ? sh.draw[turn][lane * 4 + k] : 0.0;
-    if (own[k] > 0.0) last = lane * 4 + k;
+    if (own[k] > GHOSTS) last = lane * 4 + k;
     upto += own[k];
   }
   double before = upto;
@@ -389,7 +609,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int a
   double ahead = before, at_owner = 0.0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    if (owner == INT_MAX && own[k] > 0.0 && ahead + own[k] > goal) {
+    if (owner == INT_MAX && own[k] > GHOSTS && ahead + own[k] > goal) {
       owner = lane * 4 + k;
       at_owner = ahead;
     }
@@ -399,13 +619,27 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int a
   const bool end = chosen == INT_MAX;  // a uniform at the very end, or out of range: the last id with a share
   const int winner = end ? __reduce_max_sync(FULL, last) : chosen;
   before = __shfl_sync(FULL, at_owner, (winner >> 2) & 31);
-  if (winner == rank * VERIFY_WARPS + warp) {
+  if (winner == rank * WARPS + warp) {
+    // the group first (the last one with a share where the goal is not passed), then the id
+    int g = -1;
+    {
+      double ahead = before;
+      for (int k = 0, g0 = from; k < DRAW_GROUPS && g0 < to; ++k, g0 += group) {
+        const double x = sh.group[turn][warp][k];
+        if (x > GHOSTS) g = k, before = ahead;
+        if (x > GHOSTS && ahead + x > goal && !end) break;
+        ahead += x;
+      }
+    }
     int found = -1, final = -1;
-    for (int c0 = from; c0 < to && found < 0; c0 += 32) {
+    const int g_from = from + max(g, 0) * group, g_to = min(to, g_from + group);
+    for (int c0 = g_from; c0 < g_to && found < 0; c0 += 32) {
       const int c = c0 + lane;
       double x[N], mine = 0.0;
-      if (c < to) {
-        piece_shares(c, residual, x);
+      if (c < g_to) {
+        Piece<N> p;
+        fetch(c, residual, p);
+        shares(p, residual, x);
 #pragma unroll
         for (int e = 0; e < N; ++e) mine += x[e];
       }
@@ -418,11 +652,11 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int a
       const double all = __shfl_sync(FULL, up, 31);
       double reach = before + (up - mine);
       int hit = INT_MAX, high = -1;
-      if (c < to) {
+      if (c < g_to) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           reach += x[e];
-          if (x[e] > 0.0) {
+          if (x[e] > GHOST) {
             high = row.start(c) + e;
             if (hit == INT_MAX && reach > goal) hit = high;
           }
@@ -433,24 +667,17 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) k_verify(VerifyDev v, int a
       if (lowest != INT_MAX && !end) found = lowest;
       before += all;
     }
-    // the order of summing may leave the border a rounding beyond the run's last id
+    // the order of summing may leave the border a rounding beyond the group's last id
     if (lane == 0) out[kept] = (uint32_t)(found >= 0 ? found : final);
   }
   cluster.sync();
 }
 
-cudaError_t verify_drafts(const VerifyDev& v, cudaStream_t st) {
-  if (v.sequences == 0) return cudaSuccess;
-  const int size = v.dtype == DTYPE_F32 ? 4 : 2;
-  // CTAs for a sequence: until the 148 SMs hold two each, or a slice is 8 KB
-  int ranks = 1;
-  while (ranks < VERIFY_MAX_CLUSTER && v.sequences * ranks * 2 <= 2 * 148 && v.vocab * size / ranks > 8192) ranks *= 2;
-  // rows of a round: until a CTA has 32 KB in flight
-  int at_once = 1;
-  while (at_once < VERIFY_MAX_ROWS && at_once < v.drafts + 1 && (long long)v.vocab * size / ranks * at_once * 2 <= 32768) at_once *= 2;
+template <typename T>
+static cudaError_t verify_launch(const VerifyDev& v, int ranks, int warps, int at_once, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(v.sequences * ranks));
-  cfg.blockDim = dim3(VERIFY_THREADS);
+  cfg.blockDim = dim3((unsigned)(warps * 32));
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -458,10 +685,29 @@ cudaError_t verify_drafts(const VerifyDev& v, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const bool greedy = v.temperature == 0.0f;
-  if (v.dtype == DTYPE_F32) return cudaLaunchKernelEx(&cfg, greedy ? k_verify<float, true> : k_verify<float, false>, v, at_once);
-  if (v.dtype == DTYPE_F16) return cudaLaunchKernelEx(&cfg, greedy ? k_verify<__half, true> : k_verify<__half, false>, v, at_once);
-  return cudaLaunchKernelEx(&cfg, greedy ? k_verify<__nv_bfloat16, true> : k_verify<__nv_bfloat16, false>, v, at_once);
+  if (v.temperature == 0.0f) return cudaLaunchKernelEx(&cfg, warps == 16 ? k_verify<T, true, 16> : k_verify<T, true, 8>, v, at_once);
+  return cudaLaunchKernelEx(&cfg, warps == 16 ? k_verify<T, false, 16> : k_verify<T, false, 8>, v, at_once);
+}
+
+cudaError_t verify_drafts(const VerifyDev& v, cudaStream_t st) {
+  if (v.sequences == 0) return cudaSuccess;
+  const int size = v.dtype == DTYPE_F32 ? 4 : 2;
+  // About 480 CTAs of 8 warps, up to 8 for a sequence (96 rows of 129283: 5 CTAs
+  // 95 us, 4 101, 2 154, 8 115; 256 of 8192: 2 CTAs 36 us, 1 40, 4 47); where
+  // that leaves SMs empty, of 16 warps.
+  const int n = v.sequences;
+  int ranks = (480 + n / 2) / n, warps = 8;
+  ranks = ranks < 1 ? 1 : ranks > VERIFY_MAX_CLUSTER ? VERIFY_MAX_CLUSTER : ranks;
+  if (n * ranks <= 148) warps = 16;
+  // Rows of a round: two, or more where a CTA's slices of them are 16 KB at
+  // most (one sequence of 8192: 4 rows 12.5 us, 2 16.1; a row read in vain
+  // costs less than a round of its own).
+  const long long slice = (long long)v.vocab * size / ranks;
+  int at_once = 1;
+  while (at_once < VERIFY_MAX_ROWS && at_once < v.drafts + 1 && (at_once == 1 || slice * at_once < 16384)) at_once *= 2;
+  if (v.dtype == DTYPE_F32) return verify_launch<float>(v, ranks, warps, at_once, st);
+  if (v.dtype == DTYPE_F16) return verify_launch<__half>(v, ranks, warps, at_once, st);
+  return verify_launch<__nv_bfloat16>(v, ranks, warps, at_once, st);
 }
 
 }  // namespace nbk
