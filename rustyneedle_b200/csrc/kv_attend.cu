@@ -25,28 +25,79 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 16 query rows of one kv head against a part of the prefix (PREFIX) or of a
+// 16 query rows of one kv head against a chunk of the prefix (PREFIX) or of a
 // sequence's tail. A row is (token, query head of the group): row r of a tile
-// list stands for token r / group. Four warps take the part's keys 32 at a
+// list stands for token r / group. Four warps take the chunk's keys 32 at a
 // time in turn and are joined at the end.
+//
+// The codes come by bulk copies into a ring of ATT_STAGES x 32 keys for each
+// warp (one lane asks for them, two groups ahead): 2 D + 8 bytes a key, and
+// the kernel is to be bound by those bytes. At D = 64 four CTAs an SM hold 140
+// KB in flight.
 //
 // Lanes: g = lane / 4, c = lane % 4. The key fragment of a 16 x 8 x 16 product
 // wants, of key "n = g", four dimensions of the lane's own choice for every
 // step, as long as the query fragment has the same: lane c takes 16
 // consecutive bytes of every 64, four steps of four dimensions, so a key's
-// codes arrive as one 16-byte load and need no shared memory. Product j of a
-// block of 16 keys takes the keys 4·(n / 2) + 2·j + n % 2, which leaves lane c
-// the scores of the keys 4c .. 4c + 3: the order in which the second product
-// wants its left operand, and in which the pool keeps the values (value_byte).
-constexpr int ATT_WARPS = 4;
+// codes arrive as one 16-byte load. Product j of a block of 16 keys takes the
+// keys 4·(n / 2) + 2·j + n % 2, which leaves lane c the scores of the keys 4c
+// .. 4c + 3: the order in which the second product wants its left operand, and
+// in which the pool keeps the values (value_byte).
+constexpr int ATT_WARPS = 4, ATT_STAGES = 3;
 
+template <int D>
+struct AttStage {
+  uint8_t k[32 * D];  // [D / 64][32][64]
+  uint8_t v[32 * D];
+  float ks[32], vs[32];
+};
+template <int D>
+struct AttSmem {
+  union {
+    AttStage<D> ring[ATT_WARPS][ATT_STAGES];
+    float o[ATT_WARPS][16][D + 4];  // once every copy has landed and been used
+  };
+  float2 ml[ATT_WARPS][16];
+  uint64_t full[ATT_WARPS][ATT_STAGES];
+  int failed;
+};
+
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void store_out4(const RowsDev& out, bool vector, long long at, const float (&y)[4]) {
+  uint2 w;
+  if constexpr (BF16) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(y[0], y[1]), b = __floats2bfloat162_rn(y[2], y[3]);
+    w = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+    w = make_uint2(pack_f16(y[0], y[1]), pack_f16(y[2], y[3]));
+  }
+  uint16_t* p = static_cast<uint16_t*>(out.data) + at;
+  if (vector) {
+    *reinterpret_cast<uint2*>(p) = w;
+  } else {
+    p[0] = (uint16_t)w.x;
+    p[1] = (uint16_t)(w.x >> 16);
+    p[2] = (uint16_t)w.y;
+    p[3] = (uint16_t)(w.y >> 16);
+  }
+}
+
+// FUSED (tails of one part): the prefix's parts are joined in, and the rows
+// written out.
 template <int D, bool BF16, bool E4M3, bool PREFIX>
-__global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a) {
+__global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool fused) {
   constexpr int SEG = D / 64, STEPS = D / 16, NT = D / 8;
-  __shared__ float s_o[ATT_WARPS][16][D + 1];
-  __shared__ float2 s_ml[ATT_WARPS][16];
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  AttSmem<D>& sm = *reinterpret_cast<AttSmem<D>*>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int h = blockIdx.y, part = blockIdx.z;
+  if (PREFIX) pdl_trigger();
   int token0, tokens, row0, k0, k1, sees0 = 0;  // the tile's rows row0.. of `tokens` tokens from token0; keys [k0, k1)
   const uint32_t* pages;
   if constexpr (PREFIX) {
@@ -60,19 +111,61 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a) {
     const int s = blockIdx.x / a.tiles_per_sequence;
     row0 = (blockIdx.x % a.tiles_per_sequence) * 16;
     const Span sp = span_of(a.b, s);
-    if (!sp.ok) {
-      if (threadIdx.x == 0) atomicOr(a.c.error, KV_BAD_SEQUENCE);
+    if (!sp.ok || row0 >= sp.n * a.group) {
+      if (!sp.ok && threadIdx.x == 0) atomicOr(a.c.error, KV_BAD_SEQUENCE);
+      pdl_wait();
       return;
     }
     token0 = sp.first;
     tokens = sp.n;
-    if (row0 >= tokens * a.group) return;
     sees0 = sp.len - sp.n;
     k0 = part * a.tail_chunk;
     k1 = min(sees0 + min(tokens - 1, (row0 + 15) / a.group) + 1, k0 + a.tail_chunk);
     pages = a.b.pages + (size_t)s * a.b.page_stride;
   }
   const int rows = tokens * a.group;
+  // this warp's groups of 32 keys: k0 + 32 (warp + 4 i), i < count
+  const int groups = max(0, (k1 - k0 + 31) / 32), count = max(0, (groups - warp + ATT_WARPS - 1) / ATT_WARPS);
+  if (lane == 0)
+    for (int i = 0; i < ATT_STAGES; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&sm.full[warp][i])) : "memory");
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if (threadIdx.x == 0) sm.failed = 0;
+  // the pages of the next 32 groups, one a lane
+  uint32_t held = 0;
+  int held_from = -32;
+  auto page_of = [&](int i) {  // by all lanes, with the same i
+    if (i >= held_from + 32) {
+      held_from = i;
+      held = i + lane < count ? pages[(k0 + 32 * (warp + ATT_WARPS * (i + lane))) / KV_PAGE] : 0;
+    }
+    return __shfl_sync(FULL, held, i - held_from);
+  };
+  uint32_t bad = 0;  // bit i % 32: group i's page is outside the pool
+  auto ask = [&](int i) {
+    const uint32_t page = page_of(i);
+    const bool ok = page < a.c.pages;
+    bad = (bad & ~(1u << (i & 31))) | (ok ? 0u : 1u << (i & 31));
+    if (lane == 0) {
+      AttStage<D>& st = sm.ring[warp][i % ATT_STAGES];
+      const uint32_t bar = smem_u32(&sm.full[warp][i % ATT_STAGES]);
+      if (ok) {
+        const size_t block = (size_t)page * a.c.kv_heads + h;
+        const int in_page = (k0 + 32 * (warp + ATT_WARPS * i)) % KV_PAGE;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(64 * D + 256) : "memory");
+#pragma unroll
+        for (int seg = 0; seg < SEG; ++seg)
+          bulk_copy(st.k + seg * 2048, a.c.k + block * (KV_PAGE * D) + seg * (KV_PAGE * 64) + in_page * 64, 2048, bar);
+        bulk_copy(st.v, a.c.v + block * (KV_PAGE * D) + in_page * D, 32 * D, bar);
+        bulk_copy(st.ks, a.c.ks + block * KV_PAGE + in_page, 128, bar);
+        bulk_copy(st.vs, a.c.vs + block * KV_PAGE + in_page, 128, bar);
+      } else {
+        atomicOr(a.c.error, KV_BAD_PAGE);
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+      }
+    }
+  };
+  __syncwarp();
+  for (int i = 0; i < min(count, ATT_STAGES); ++i) ask(i);
 
   // the lane's query fragments; rows past the end are zeros
   uint32_t qf[STEPS][4];
@@ -106,166 +199,215 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a) {
 
   float o[NT][4] = {};
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-  for (int kb = k0 + 32 * warp; kb < k1; kb += 32 * ATT_WARPS) {
-    const uint32_t page = pages[kb / KV_PAGE];
-    if (page >= a.c.pages) {
-      if (lane == 0) atomicOr(a.c.error, KV_BAD_PAGE);
-      continue;
-    }
-    const size_t block = (size_t)page * a.c.kv_heads + h;
-    const int in_page = kb % KV_PAGE;
-    const uint8_t* kp = a.c.k + block * (KV_PAGE * D) + in_page * D;
-    const uint8_t* vp = a.c.v + block * (KV_PAGE * D) + in_page * D;
-    float t[2][2][4];  // [block of 16 keys][product][row g: two keys, row g + 8: two keys]
-    float inv[2][4];   // 1 / vs of the keys 4c .. 4c + 3
+  bool fine = true;
+  for (int i = 0; i < count; ++i) {
+    const int kb = k0 + 32 * (warp + ATT_WARPS * i);
+    fine = fine && __all_sync(FULL, mbar_wait_polls(smem_u32(&sm.full[warp][i % ATT_STAGES]), (i / ATT_STAGES) & 1, 1u << 18));
+    if (!fine) break;
+    const AttStage<D>& stage = sm.ring[warp][i % ATT_STAGES];
+    if (!(bad >> (i & 31) & 1)) {
+      float t[2][2][4];  // [block of 16 keys][product][row g: two keys, row g + 8: two keys]
+      float inv[2][4];   // 1 / vs of the keys 4c .. 4c + 3
 #pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-      const float4 ks = *reinterpret_cast<const float4*>(a.c.ks + block * KV_PAGE + in_page + blk * 16 + c * 4);
-      const float4 vs = *reinterpret_cast<const float4*>(a.c.vs + block * KV_PAGE + in_page + blk * 16 + c * 4);
-      const float kscale[4] = {ks.x, ks.y, ks.z, ks.w}, vscale[4] = {vs.x, vs.y, vs.z, vs.w};
+      for (int blk = 0; blk < 2; ++blk) {
+        const float4 ks = *reinterpret_cast<const float4*>(stage.ks + blk * 16 + c * 4);
+        const float4 vs = *reinterpret_cast<const float4*>(stage.vs + blk * 16 + c * 4);
+        const float kscale[4] = {ks.x, ks.y, ks.z, ks.w}, vscale[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float s[4] = {};
-        const uint8_t* row = kp + (blk * 16 + 4 * (g >> 1) + 2 * j + (g & 1)) * D + c * 16;
+        for (int j = 0; j < 2; ++j) {
+          float s[4] = {};
+          const uint8_t* row = stage.k + (blk * 16 + 4 * (g >> 1) + 2 * j + (g & 1)) * 64 + c * 16;
 #pragma unroll
-        for (int seg = 0; seg < SEG; ++seg) {
-          const uint4 w = *reinterpret_cast<const uint4*>(row + seg * 64);
+          for (int seg = 0; seg < SEG; ++seg) {
+            const uint4 w = *reinterpret_cast<const uint4*>(row + seg * 2048);
+            const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+              const uint2 kf = widen<E4M3, BF16>(word[st]);
+              mma16816<BF16>(s, qf[seg * 4 + st], kf.x, kf.y);
+            }
+          }
+#pragma unroll
+          for (int e2 = 0; e2 < 2; ++e2) {
+            const int e = 2 * j + e2, key = kb + blk * 16 + 4 * c + e;
+            const float mul = __fmul_rn(kscale[e], a.scale), add = lg2(vscale[e]);
+            inv[blk][e] = key < k1 ? rcp_fast(vscale[e]) : 0.0f;
+            // a key that a row does not see gets -inf by selection, whatever lies there
+            t[blk][j][e2] = key < limit[0] ? __fmaf_rn(s[e2], mul, add) : -INFINITY;
+            t[blk][j][2 + e2] = key < limit[1] ? __fmaf_rn(s[2 + e2], mul, add) : -INFINITY;
+          }
+        }
+      }
+      float base[2];
+      bool grown = false;
+      float next[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(t[blk][j][2 * half], t[blk][j][2 * half + 1]));
+        top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+        next[half] = fmaxf(m[half], __fadd_rn(top, -HEADROOM));
+        grown = grown || next[half] != m[half];
+        base[half] = next[half] == -INFINITY ? 0.0f : next[half];
+      }
+      if (__any_sync(FULL, grown)) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float keep = ex2(__fadd_rn(m[half], -base[half]));  // 0 while nothing was seen
+          m[half] = next[half];
+          l[half] = __fmul_rn(l[half], keep);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            o[n][2 * half] = __fmul_rn(o[n][2 * half], keep);
+            o[n][2 * half + 1] = __fmul_rn(o[n][2 * half + 1], keep);
+          }
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {
+              float& x = t[blk][j][2 * half + e2];
+              const bool seen = x != -INFINITY;
+              x = ex2(__fadd_rn(x, -base[half]));
+              l[half] = seen ? __fmaf_rn(x, inv[blk][2 * j + e2], l[half]) : l[half];
+            }
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        const uint32_t pf[4] = {pack_f16(t[blk][0][0], t[blk][0][1]), pack_f16(t[blk][0][2], t[blk][0][3]), pack_f16(t[blk][1][0], t[blk][1][1]),
+                                pack_f16(t[blk][1][2], t[blk][1][3])};
+#pragma unroll
+        for (int tq = 0; tq < D / 32; ++tq) {
+          const uint4 w = *reinterpret_cast<const uint4*>(stage.v + blk * 16 * D + tq * 512 + lane * 16);
           const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int st = 0; st < 4; ++st) {
-            const uint2 kf = widen<E4M3, BF16>(word[st]);
-            mma16816<BF16>(s, qf[seg * 4 + st], kf.x, kf.y);
+          for (int n = 0; n < 4; ++n) {
+            const uint2 vf = widen<E4M3, false>(word[n]);
+            mma16816<false>(o[tq * 4 + n], pf, vf.x, vf.y);
           }
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int e = 2 * j + i, key = kb + blk * 16 + 4 * c + e;
-          const float mul = __fmul_rn(kscale[e], a.scale), add = lg2(vscale[e]);
-          inv[blk][e] = key < k1 ? __frcp_rn(vscale[e]) : 0.0f;
-          // a key that a row does not see gets -inf by selection, whatever lies there
-          t[blk][j][i] = key < limit[0] ? __fmaf_rn(s[i], mul, add) : -INFINITY;
-          t[blk][j][2 + i] = key < limit[1] ? __fmaf_rn(s[2 + i], mul, add) : -INFINITY;
-        }
       }
     }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(t[blk][j][2 * half], t[blk][j][2 * half + 1]));
-      top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
-      const float next = fmaxf(m[half], __fadd_rn(top, -HEADROOM));
-      const float base = next == -INFINITY ? 0.0f : next;
-      const float keep = ex2(__fadd_rn(m[half], -base));  // 0 while nothing was seen
-      m[half] = next;
-      float sum = 0.0f;
-#pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float& x = t[blk][j][2 * half + i];
-            const bool seen = x != -INFINITY;
-            x = ex2(__fadd_rn(x, -base));
-            sum = seen ? __fmaf_rn(x, inv[blk][2 * j + i], sum) : sum;
-          }
-      l[half] = __fmaf_rn(l[half], keep, sum);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        o[n][2 * half] = __fmul_rn(o[n][2 * half], keep);
-        o[n][2 * half + 1] = __fmul_rn(o[n][2 * half + 1], keep);
-      }
-    }
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-      const uint32_t pf[4] = {pack_f16(t[blk][0][0], t[blk][0][1]), pack_f16(t[blk][0][2], t[blk][0][3]), pack_f16(t[blk][1][0], t[blk][1][1]),
-                              pack_f16(t[blk][1][2], t[blk][1][3])};
-#pragma unroll
-      for (int tq = 0; tq < D / 32; ++tq) {
-        const uint4 w = *reinterpret_cast<const uint4*>(vp + blk * 16 * D + tq * 512 + g * 64 + c * 16);
-        const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const uint2 vf = widen<E4M3, false>(word[n]);
-          mma16816<false>(o[tq * 4 + n], pf, vf.x, vf.y);
-        }
-      }
-    }
+    __syncwarp();
+    if (i + ATT_STAGES < count) ask(i + ATT_STAGES);
+  }
+  if (!fine && lane == 0) {  // what was asked for lands before the block ends
+    sm.failed = 1;
+    atomicOr(a.c.error, KV_WAIT_FAILED);
+    for (int i = 0; i < min(count, ATT_STAGES); ++i) mbar_wait_polls(smem_u32(&sm.full[warp][i]), 1, 1u << 18), mbar_wait_polls(smem_u32(&sm.full[warp][i]), 0, 1u << 18);
   }
 
-  // join the four warps: rows of a common maximum
+  // join the four warps, the ring's memory holding their accumulators
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     l[half] = __fadd_rn(l[half], __shfl_xor_sync(FULL, l[half], 1));
     l[half] = __fadd_rn(l[half], __shfl_xor_sync(FULL, l[half], 2));
-    if (c == 0) s_ml[warp][g + 8 * half] = make_float2(m[half], l[half]);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      s_o[warp][g + 8 * half][n * 8 + 2 * c] = o[n][2 * half];
-      s_o[warp][g + 8 * half][n * 8 + 2 * c + 1] = o[n][2 * half + 1];
-    }
+    if (c == 0) sm.ml[warp][g + 8 * half] = make_float2(m[half], l[half]);
   }
   __syncthreads();
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(&sm.o[warp][g + 8 * half][n * 8 + 2 * c]) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
+  pdl_wait();  // the prefix's parts are complete (and whatever the launch before wrote)
+  __syncthreads();
+  if (sm.failed) return;
   const int index = PREFIX ? part : a.prefix_parts + part;
-  for (int x = threadIdx.x; x < 16 * D; x += ATT_WARPS * 32) {
-    const int r = x / D, d = x % D;
+  const size_t stride = (size_t)a.b.rows * a.heads;
+  for (int x = threadIdx.x; x < 16 * D / 4; x += ATT_WARPS * 32) {
+    const int r = x / (D / 4), d = x % (D / 4) * 4;
     if (row0 + r >= rows) break;
+    const size_t unit = (size_t)(token0 + (row0 + r) / a.group) * a.heads + h * a.group + (row0 + r) % a.group;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < ATT_WARPS; ++w) top = fmaxf(top, s_ml[w][r].x);
+    for (int w = 0; w < ATT_WARPS; ++w) top = fmaxf(top, sm.ml[w][r].x);
+    if (fused)
+      for (int p = 0; p < a.prefix_parts; ++p) top = fmaxf(top, __ldcg(&a.part_ml[p * stride + unit].x));
     const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, value = 0.0f;
+    float sum = 0.0f, y[4] = {};
 #pragma unroll
     for (int w = 0; w < ATT_WARPS; ++w) {
-      const float f = ex2(__fadd_rn(s_ml[w][r].x, -base));
-      sum = __fmaf_rn(s_ml[w][r].y, f, sum);
-      value = __fmaf_rn(s_o[w][r][d], f, value);
+      const float f = ex2(__fadd_rn(sm.ml[w][r].x, -base));
+      const float4 v = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
+      sum = __fmaf_rn(sm.ml[w][r].y, f, sum);
+      y[0] = __fmaf_rn(v.x, f, y[0]);
+      y[1] = __fmaf_rn(v.y, f, y[1]);
+      y[2] = __fmaf_rn(v.z, f, y[2]);
+      y[3] = __fmaf_rn(v.w, f, y[3]);
     }
-    const size_t at = ((size_t)index * a.b.rows + token0 + (row0 + r) / a.group) * a.heads + h * a.group + (row0 + r) % a.group;
-    a.part_o[at * D + d] = value;
-    if (d == 0) a.part_ml[at] = make_float2(top, sum);
+    if (!fused) {
+      const size_t at = index * stride + unit;
+      *reinterpret_cast<float4*>(a.part_o + at * D + d) = make_float4(y[0], y[1], y[2], y[3]);
+      if (d == 0) a.part_ml[at] = make_float2(top, sum);
+      continue;
+    }
+#pragma unroll 4
+    for (int p = 0; p < a.prefix_parts; ++p) {
+      const float2 ml = __ldcg(&a.part_ml[p * stride + unit]);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + (p * stride + unit) * D + d));
+      const float f = ex2(__fadd_rn(ml.x, -base));
+      sum = __fmaf_rn(ml.y, f, sum);
+      y[0] = __fmaf_rn(v.x, f, y[0]);
+      y[1] = __fmaf_rn(v.y, f, y[1]);
+      y[2] = __fmaf_rn(v.z, f, y[2]);
+      y[3] = __fmaf_rn(v.w, f, y[3]);
+    }
+    const float norm = sum == 0.0f ? 0.0f : __frcp_rn(sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(y[e], norm);
+    const int row = token0 + (row0 + r) / a.group, head = h * a.group + (row0 + r) % a.group;
+    store_out4<BF16>(a.out, a.out_vector, row * a.out.row_stride + head * a.out.head_stride + d, y);
   }
 }
 
-// Joins the parts of a row: one warp for each (token, head).
+// Joins the parts of a row: D / 4 lanes for each (token, head).
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) k_kv_join(AttendDev a) {
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x & 31;
-  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (unit >= (long long)a.b.rows * a.heads) return;
-  const int row = (int)(unit / a.heads), head = (int)(unit % a.heads);
-  const int s = sequence_of(a.b, row);
+  constexpr int LANES = D / 4;
+  pdl_wait();
+  const int lane = threadIdx.x % LANES;
+  const long long unit = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;
+  const bool some = unit < (long long)a.b.rows * a.heads;
+  const int row = some ? (int)(unit / a.heads) : 0, head = some ? (int)(unit % a.heads) : 0;
+  // all of a warp's units are of the first one's row or of rows behind it: search for each row that occurs
+  int s = 0;
+  for (unsigned left = __ballot_sync(FULL, true); left;) {
+    const int one = __shfl_sync(FULL, row, __ffs(left) - 1);
+    const int found = sequence_of(a.b, one);
+    if (row == one) s = found;
+    left &= ~__ballot_sync(FULL, row == one);
+  }
   const Span sp = span_of(a.b, s);
-  if (!sp.ok || row < sp.first || row >= sp.first + sp.n) return;
+  if (!some || !sp.ok || row < sp.first || row >= sp.first + sp.n) return;
   const int parts = a.prefix_parts + a.tail_parts;
   const size_t stride = (size_t)a.b.rows * a.heads;
   float top = -INFINITY;
   for (int p = 0; p < parts; ++p) top = fmaxf(top, a.part_ml[p * stride + unit].x);
   const float base = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, x[N] = {};
+  float sum = 0.0f, y[4] = {};
+#pragma unroll 4
   for (int p = 0; p < parts; ++p) {
     const float2 ml = a.part_ml[p * stride + unit];
+    const float4 v = *reinterpret_cast<const float4*>(a.part_o + (p * stride + unit) * D + lane * 4);
     const float f = ex2(__fadd_rn(ml.x, -base));
     sum = __fmaf_rn(ml.y, f, sum);
-    const float* o = a.part_o + (p * stride + unit) * D + lane * N;
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = __fmaf_rn(o[i], f, x[i]);
+    y[0] = __fmaf_rn(v.x, f, y[0]);
+    y[1] = __fmaf_rn(v.y, f, y[1]);
+    y[2] = __fmaf_rn(v.z, f, y[2]);
+    y[3] = __fmaf_rn(v.w, f, y[3]);
   }
   const float norm = sum == 0.0f ? 0.0f : __frcp_rn(sum);
-  const long long at = row * a.out.row_stride + head * a.out.head_stride + lane * N;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float y = __fmul_rn(x[i], norm);
-    if constexpr (BF16)
-      static_cast<__nv_bfloat16*>(a.out.data)[at + i] = __float2bfloat16_rn(y);
-    else
-      static_cast<__half*>(a.out.data)[at + i] = __float2half_rn(y);
-  }
+  for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(y[e], norm);
+  store_out4<BF16>(a.out, a.out_vector, row * a.out.row_stride + head * a.out.head_stride + lane * 4, y);
 }
 
 // How a side (the prefix or the tails) is cut: the kernel, its row tiles and
@@ -333,25 +475,51 @@ size_t kv_attend_workspace(const KvCacheDev& c, const KvBatchDev& b, int prefix,
   return units * (c.dim * sizeof(float) + sizeof(float2)) + 16;
 }
 
+template <typename... P, typename... A>
+static cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, bool dependent, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// The first launch waits for all before it on the stream (the keys and queries
+// may just have been written). The ones behind it start early: they read
+// nothing of their predecessor before pdl_wait(), and a launch completes only
+// after its own pdl_wait(), so the last one finds every part.
 template <int D, bool BF16, bool E4M3>
 static cudaError_t attend_launch(const AttendDev& d, const AttendPlan& p, cudaStream_t st) {
-  cudaError_t e = cudaSuccess;
-  if (p.prefix.chunks) {
+  constexpr int SMEM = (int)sizeof(AttSmem<D>);
+  cudaError_t e = cudaFuncSetAttribute(k_kv_attend<D, BF16, E4M3, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(k_kv_attend<D, BF16, E4M3, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  bool before = false;  // a launch of this call goes before
+  if (e == cudaSuccess && p.prefix.chunks) {
     if (p.prefix.wide)
-      e = attend_wide(d, true, p.prefix.tiles, p.prefix.chunks, st);
+      e = attend_wide(d, true, p.prefix.tiles, p.prefix.chunks, false, st);
     else
-      k_kv_attend<D, BF16, E4M3, true><<<dim3(p.prefix.tiles, d.c.kv_heads, p.prefix.chunks), ATT_WARPS * 32, 0, st>>>(d);
+      e = launch(k_kv_attend<D, BF16, E4M3, true>, dim3(p.prefix.tiles, d.c.kv_heads, p.prefix.chunks), ATT_WARPS * 32, SMEM, false, st, d, false);
+    before = true;
   }
+  bool fused = false;
   if (e == cudaSuccess && p.tail.chunks) {
     const unsigned tiles = (unsigned)d.b.sequences * p.tail.tiles;
+    fused = !p.tail.wide && p.tail.parts == 1;
     if (p.tail.wide)
-      e = attend_wide(d, false, (int)tiles, p.tail.chunks, st);
+      e = attend_wide(d, false, (int)tiles, p.tail.chunks, before, st);
     else
-      k_kv_attend<D, BF16, E4M3, false><<<dim3(tiles, d.c.kv_heads, p.tail.chunks), ATT_WARPS * 32, 0, st>>>(d);
+      e = launch(k_kv_attend<D, BF16, E4M3, false>, dim3(tiles, d.c.kv_heads, p.tail.chunks), ATT_WARPS * 32, SMEM, before, st, d, fused);
+    before = true;
   }
-  if (e != cudaSuccess) return e;
-  k_kv_join<D, BF16><<<(unsigned)(((long long)d.b.rows * d.heads + 7) / 8), 256, 0, st>>>(d);
-  return cudaGetLastError();
+  if (e == cudaSuccess && !fused)
+    e = launch(k_kv_join<D, BF16>, dim3((unsigned)(((long long)d.b.rows * d.heads * (D / 4) + 255) / 256)), 256, 0, before, st, d);
+  return e;
 }
 
 cudaError_t kv_attend(const KvCacheDev& c, const KvBatchDev& b, const KvAttend& x, cudaStream_t st) {
@@ -369,6 +537,7 @@ cudaError_t kv_attend(const KvCacheDev& c, const KvBatchDev& b, const KvAttend& 
   d.out = x.out;
   d.q_vector = reinterpret_cast<uintptr_t>(x.query.data) % 8 == 0 && x.query.row_stride % 4 == 0 && x.query.head_stride % 4 == 0;
   d.q_vector16 = reinterpret_cast<uintptr_t>(x.query.data) % 16 == 0 && x.query.row_stride % 8 == 0 && x.query.head_stride % 8 == 0;
+  d.out_vector = reinterpret_cast<uintptr_t>(x.out.data) % 8 == 0 && x.out.row_stride % 4 == 0 && x.out.head_stride % 4 == 0;
   d.prefix_parts = p.prefix.parts;
   d.prefix_chunk = p.prefix.chunk;
   d.prefix_pair = p.prefix.pair;

@@ -15,7 +15,7 @@ struct AttendDev {
   int prefix, heads, group;
   float scale;  // softmax scale · log2 e
   RowsDev q, out;
-  bool q_vector, q_vector16;  // rows may be read 8 (16) bytes at a time
+  bool q_vector, q_vector16, out_vector;  // rows may be read 8 (16), written 8 bytes at a time
   float* part_o;  // [parts][rows][heads][dim], unnormalised
   float2* part_ml;  // [parts][rows][heads]: maximum (less HEADROOM) and sum
   int prefix_parts, tail_parts;  // parts of a row
@@ -42,6 +42,7 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 
 // The kernel for many rows (kv_attend_wide.cu) over the prefix or the tails:
 // `tiles` 128-row tiles, or pairs of them, times kv_heads times chunks CTAs.
-cudaError_t attend_wide(const AttendDev& a, bool prefix, int tiles, int chunks, cudaStream_t st);
+// `dependent`: it follows another launch of the same call.
+cudaError_t attend_wide(const AttendDev& a, bool prefix, int tiles, int chunks, bool dependent, cudaStream_t st);
 
 }  // namespace nbk

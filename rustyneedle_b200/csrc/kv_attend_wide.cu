@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int h = blockIdx.y, part = blockIdx.z, cover = pair ? 2 * WIDE_ROWS : WIDE_ROWS;
 
+  pdl_trigger();  // a launch that may follow starts as SMs become free; it waits for this one where it joins
   int token0, tokens, row0, k0, k1, sees0 = 0;
   const uint32_t* pages;
   if (prefix) {
@@ -126,13 +127,13 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
     const int s = blockIdx.x / a.tiles_per_sequence;
     row0 = (blockIdx.x % a.tiles_per_sequence) * cover;
     const Span sp = span_of(a.b, s);
-    if (!sp.ok) {
-      if (tid == 0) atomicOr(a.c.error, KV_BAD_SEQUENCE);
+    if (!sp.ok || row0 >= sp.n * a.group) {
+      if (!sp.ok && tid == 0) atomicOr(a.c.error, KV_BAD_SEQUENCE);
+      pdl_wait();
       return;
     }
     token0 = sp.first;
     tokens = sp.n;
-    if (row0 >= tokens * a.group) return;
     sees0 = sp.len - sp.n;
     k0 = part * a.tail_chunk;
     k1 = min(sees0 + min(tokens - 1, (row0 + cover - 1) / a.group) + 1, k0 + a.tail_chunk);
@@ -322,12 +323,12 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
           page_ok = true;
           const size_t block = (size_t)page * a.c.kv_heads + h;
           const int in_page = key0 % KV_PAGE;
-          const uint8_t* kp = a.c.k + block * (KV_PAGE * D) + in_page * D;
+          const uint8_t* kp = a.c.k + block * (KV_PAGE * D) + in_page * 64;
           const uint8_t* vp = a.c.v + block * (KV_PAGE * D) + in_page * D;
           // 8 keys x 4 pieces of 16 codes a load
 #pragma unroll
           for (int x = 0; x < KN; ++x)
-            kr[x] = *reinterpret_cast<const uint4*>(kp + ((x / (D / 64)) * 8 + (lane & 7)) * D + (x % (D / 64)) * 64 + (lane >> 3) * 16);
+            kr[x] = *reinterpret_cast<const uint4*>(kp + (x % (D / 64)) * (KV_PAGE * 64) + ((x / (D / 64)) * 8 + (lane & 7)) * 64 + (lane >> 3) * 16);
           // two blocks of 16 keys; of each, eight keys of dimension groups 8t + lane % 8
 #pragma unroll
           for (int x = 0; x < VN; ++x) {
@@ -430,6 +431,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
     }
     __syncwarp();
   }
+  pdl_wait();  // this launch is complete only after the one before it
   fence_before();
   __syncthreads();
   if (warp == 12) {
@@ -440,26 +442,34 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
 }
 
 template <int D, bool BF16, bool E4M3>
-static cudaError_t wide_launch(const AttendDev& a, bool prefix, int tiles, int chunks, cudaStream_t st) {
+static cudaError_t wide_launch(const AttendDev& a, bool prefix, int tiles, int chunks, bool dependent, cudaStream_t st) {
   static_assert(sizeof(WideSmem<D>) <= 227 * 1024, "fits an SM's shared memory");
   auto kernel = k_kv_attend_wide<D, BF16, E4M3>;
   // an attribute of the current device's context; setting it is idempotent and cheap beside the launch
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(WideSmem<D>));
   if (e != cudaSuccess) return e;
   const bool pair = prefix ? a.prefix_pair : a.tail_pair;
-  kernel<<<dim3((unsigned)tiles, (unsigned)a.c.kv_heads, (unsigned)chunks), WIDE_ATT_THREADS, sizeof(WideSmem<D>), st>>>(a, prefix, pair,
-                                                                                                               prefix ? 0 : a.prefix_parts);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)tiles, (unsigned)a.c.kv_heads, (unsigned)chunks);
+  cfg.blockDim = dim3(WIDE_ATT_THREADS);
+  cfg.dynamicSmemBytes = sizeof(WideSmem<D>);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, a, prefix, pair, prefix ? 0 : a.prefix_parts);
 }
 
-cudaError_t attend_wide(const AttendDev& a, bool prefix, int tiles, int chunks, cudaStream_t st) {
+cudaError_t attend_wide(const AttendDev& a, bool prefix, int tiles, int chunks, bool dependent, cudaStream_t st) {
   const bool bf16 = a.q.dtype == DTYPE_BF16;
   if (a.c.dim == 64) {
-    if (bf16) return a.c.e4m3 ? wide_launch<64, true, true>(a, prefix, tiles, chunks, st) : wide_launch<64, true, false>(a, prefix, tiles, chunks, st);
-    return a.c.e4m3 ? wide_launch<64, false, true>(a, prefix, tiles, chunks, st) : wide_launch<64, false, false>(a, prefix, tiles, chunks, st);
+    if (bf16) return a.c.e4m3 ? wide_launch<64, true, true>(a, prefix, tiles, chunks, dependent, st) : wide_launch<64, true, false>(a, prefix, tiles, chunks, dependent, st);
+    return a.c.e4m3 ? wide_launch<64, false, true>(a, prefix, tiles, chunks, dependent, st) : wide_launch<64, false, false>(a, prefix, tiles, chunks, dependent, st);
   }
-  if (bf16) return a.c.e4m3 ? wide_launch<128, true, true>(a, prefix, tiles, chunks, st) : wide_launch<128, true, false>(a, prefix, tiles, chunks, st);
-  return a.c.e4m3 ? wide_launch<128, false, true>(a, prefix, tiles, chunks, st) : wide_launch<128, false, false>(a, prefix, tiles, chunks, st);
+  if (bf16) return a.c.e4m3 ? wide_launch<128, true, true>(a, prefix, tiles, chunks, dependent, st) : wide_launch<128, true, false>(a, prefix, tiles, chunks, dependent, st);
+  return a.c.e4m3 ? wide_launch<128, false, true>(a, prefix, tiles, chunks, dependent, st) : wide_launch<128, false, false>(a, prefix, tiles, chunks, dependent, st);
 }
 
 }  // namespace nbk

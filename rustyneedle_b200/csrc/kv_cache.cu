@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_append(KvCacheDev c, KvBa
   const int at = p % KV_PAGE;
   const size_t block = (size_t)page * c.kv_heads + h;
   if (!value) {
-    uint8_t* dst = c.k + block * (KV_PAGE * D) + at * D + lane * N;
+    uint8_t* dst = c.k + block * (KV_PAGE * D) + key_byte(at, lane * N);
     if constexpr (N == 2)
       *reinterpret_cast<uint16_t*>(dst) = (uint16_t)(code[0] | code[1] << 8);
     else
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_read(KvCacheDev c, KvBatc
   const size_t block = (size_t)page * c.kv_heads + h;
   float x[N];
   if (!value) {
-    const uint8_t* src = c.k + block * (KV_PAGE * D) + at * D + lane * N;
+    const uint8_t* src = c.k + block * (KV_PAGE * D) + key_byte(at, lane * N);
     const float scale = c.ks[block * KV_PAGE + at];
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = __fmul_rn(code_value<E4M3>(src[i]), scale);

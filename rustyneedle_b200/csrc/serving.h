@@ -16,9 +16,9 @@ constexpr int KV_MAX_GROUP = 64;  // query heads of one kv head
 enum Dtype { DTYPE_F32 = 0, DTYPE_F16 = 1, DTYPE_BF16 = 2 };
 
 // The pool: codes [pages][kv_heads][64 · dim] and scales [pages][kv_heads][64]
-// for keys and values. Keys are rows [64][dim]. Values are stored in the order
-// in which a warp's lanes feed them to a matrix instruction: within a page and
-// head, code (position p, dimension d) is byte value_byte(p, d) below.
+// for keys and values. Within a page and head, the key code of position p and
+// dimension d is byte key_byte(p, d) below, the value code byte value_byte(p,
+// d): the orders in which a warp's lanes feed them to matrix instructions.
 struct KvCacheDev {
   uint8_t *k = nullptr, *v = nullptr;
   float *ks = nullptr, *vs = nullptr;
@@ -27,6 +27,10 @@ struct KvCacheDev {
   uint32_t pages = 0;
   bool e4m3 = false;
 };
+
+// Rows of 64 codes: eight lanes that read 16 bytes each of two neighbouring
+// rows meet in no bank of shared memory.
+__host__ __device__ constexpr int key_byte(int p, int d) { return (d / 64) * (KV_PAGE * 64) + p * 64 + d % 64; }
 
 // 16 positions × 32 dimensions make a 512-byte block of 32 lanes × 16 bytes:
 // lane 4·(d % 8) + (p % 16) / 4 holds four dimensions d % 32 / 8 of four
