@@ -8,8 +8,9 @@
 //   one tile:  the slots are one row tile over alternate key tiles.
 // While one slot's scores go through the softmax, the tensor cores work for
 // the other. Warps 0-3 and 4-7 are the slots' softmax (a thread is a row:
-// TMEM lane = row), warps 8-11 load codes and widen them into shared memory,
-// one lane of warp 12 issues the matrix instructions:
+// TMEM lane = row; a row of 128 scores stays in registers between its maximum
+// and its exponentials), warps 8-11 load codes and widen them into shared
+// memory, one lane of warp 12 issues the matrix instructions:
 //   S = Q K^T   Q and K codes (f16 or bf16) from shared memory, f32 in TMEM
 //   O += P V    P (f16) from TMEM, over the first half of S; V codes (f16)
 // O is rescaled in TMEM only when a row's maximum has grown by more than
@@ -23,7 +24,7 @@
 
 namespace nbk {
 
-constexpr int WIDE_ROWS = 128, WIDE_KEYS = 128, WIDE_ATT_THREADS = 13 * 32;
+constexpr int WIDE_ROWS = 128, WIDE_KEYS = 128, WIDE_ATT_THREADS = 16 * 32;
 constexpr int WIDE_LOADERS = 128;
 constexpr float SLACK = 6.0f;
 
@@ -89,6 +90,51 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 // Every wait here is for work of microseconds.
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t phase) { return mbar_wait_polls(bar, phase, 1u << 18); }
 
+// The launch's 512 threads hold 128 registers each; the four warpgroups share
+// them out anew as 192 + 192 + 88 + 40 = 4 x 128.
+template <int N>
+__device__ __forceinline__ void registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// One row's 128 scores t (already scaled, the value scale's logarithm added)
+// to weights 2^(t + base): packed as f16 for the product, summed over inv.
+// PARTIAL: scores of -inf are keys that the row does not see, whose inv may be
+// anything.
+template <bool PARTIAL>
+__device__ __forceinline__ float2 weigh(const float2 (&t)[64], float base, const float* inv, uint32_t p_addr, float2 sum) {
+  const float2 base2 = make_float2(base, base);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t p[16];
+#pragma unroll
+    for (int x = 0; x < 16; x += 2) {
+      float4 in = *reinterpret_cast<const float4*>(inv + c * 32 + x * 2);
+      float2 w0 = t[c * 16 + x], w1 = t[c * 16 + x + 1];
+      if (PARTIAL) {
+        in.x = w0.x == -INFINITY ? 0.0f : in.x;
+        in.y = w0.y == -INFINITY ? 0.0f : in.y;
+        in.z = w1.x == -INFINITY ? 0.0f : in.z;
+        in.w = w1.y == -INFINITY ? 0.0f : in.w;
+      }
+      w0 = add2(w0, base2);
+      w1 = add2(w1, base2);
+      w0 = make_float2(ex2(w0.x), ex2(w0.y));
+      w1 = make_float2(ex2(w1.x), ex2(w1.y));
+      sum = fma2(w0, make_float2(in.x, in.y), sum);
+      sum = fma2(w1, make_float2(in.z, in.w), sum);
+      p[x] = pack_f16(w0.x, w0.y);
+      p[x + 1] = pack_f16(w1.x, w1.y);
+    }
+    tmem_store16(p_addr + c * 16, p);
+  }
+  return sum;
+}
+
 template <int D>
 struct WideSmem {
   uint8_t q[2][WIDE_ROWS * D * 2];   // [slot or 0] rows x D
@@ -102,7 +148,7 @@ struct WideSmem {
   int failed;
 };
 
-// grid (row tiles (or pairs) x sequences, kv heads, parts), block 416
+// grid (row tiles (or pairs) x sequences, kv heads, chunks), block 512
 template <int D, bool BF16, bool E4M3>
 __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDev a, bool prefix, bool pair, int parts0) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -188,6 +234,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
   bool ok = true;
   if (warp < 8) {
     // ------------------------------------------------------------- softmax
+    registers_up<192>();
     const int slot = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + slot * 128, o_addr = tmem + lanes + 256 + slot * 128;
@@ -207,28 +254,42 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
       const float* add = sm.add[j & 3];
       const float* inv = sm.inv[j & 3];
       const bool partial = key0 + WIDE_KEYS > all_see && !prefix;
-      float top = -INFINITY;
-#pragma unroll 1
-      for (int c = 0; c < WIDE_KEYS; c += 32) {
-        uint32_t s[32];
-        tmem_load32(s_addr + c, s);
+      float2 t[64];
+      {
+        uint32_t r0[32], r1[32], r2[32], r3[32];
+        tmem_load32(s_addr, r0);
+        tmem_load32(s_addr + 32, r1);
+        tmem_load32(s_addr + 64, r2);
+        tmem_load32(s_addr + 96, r3);
         tmem_wait_load();
 #pragma unroll
-        for (int x = 0; x < 32; x += 4) {
-          const float4 mu = *reinterpret_cast<const float4*>(mul + c + x), ad = *reinterpret_cast<const float4*>(add + c + x);
-          float2 t0 = fma2(make_float2(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), make_float2(mu.x, mu.y), make_float2(ad.x, ad.y));
-          float2 t1 = fma2(make_float2(__uint_as_float(s[x + 2]), __uint_as_float(s[x + 3])), make_float2(mu.z, mu.w), make_float2(ad.z, ad.w));
-          if (partial) {
-            const int k = key0 + c + x;
-            t0.x = k < limit ? t0.x : -INFINITY;
-            t0.y = k + 1 < limit ? t0.y : -INFINITY;
-            t1.x = k + 2 < limit ? t1.x : -INFINITY;
-            t1.y = k + 3 < limit ? t1.y : -INFINITY;
-          }
-          top = fmaxf(top, fmaxf(fmaxf(t0.x, t0.y), fmaxf(t1.x, t1.y)));
+        for (int x = 0; x < 16; ++x) {
+          t[x] = make_float2(__uint_as_float(r0[2 * x]), __uint_as_float(r0[2 * x + 1]));
+          t[16 + x] = make_float2(__uint_as_float(r1[2 * x]), __uint_as_float(r1[2 * x + 1]));
+          t[32 + x] = make_float2(__uint_as_float(r2[2 * x]), __uint_as_float(r2[2 * x + 1]));
+          t[48 + x] = make_float2(__uint_as_float(r3[2 * x]), __uint_as_float(r3[2 * x + 1]));
         }
       }
-      const float want = __fadd_rn(top, -HEADROOM);
+      float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 64; x += 2) {
+        const float4 mu = *reinterpret_cast<const float4*>(mul + 2 * x), ad = *reinterpret_cast<const float4*>(add + 2 * x);
+        t[x] = fma2(t[x], make_float2(mu.x, mu.y), make_float2(ad.x, ad.y));
+        t[x + 1] = fma2(t[x + 1], make_float2(mu.z, mu.w), make_float2(ad.z, ad.w));
+      }
+      if (partial) {
+#pragma unroll
+        for (int x = 0; x < 64; ++x) {
+          t[x].x = key0 + 2 * x < limit ? t[x].x : -INFINITY;
+          t[x].y = key0 + 2 * x + 1 < limit ? t[x].y : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 64; x += 2) {
+        top0 = fmaxf(top0, fmaxf(t[x].x, t[x].y));
+        top1 = fmaxf(top1, fmaxf(t[x + 1].x, t[x + 1].y));
+      }
+      const float want = __fadd_rn(fmaxf(top0, top1), -HEADROOM);
       const bool grown = want > __fadd_rn(m, SLACK) || m == -INFINITY;
       if (__any_sync(FULL, grown)) {
         const float next = grown ? fmaxf(m, want) : m;
@@ -248,36 +309,8 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
         }
       }
       const float base = m == -INFINITY ? 0.0f : -m;
-      const float2 base2 = make_float2(base, base);
-#pragma unroll 1
-      for (int c = 0; c < WIDE_KEYS; c += 32) {
-        uint32_t s[32], p[16];
-        tmem_load32(s_addr + c, s);
-        tmem_wait_load();
-#pragma unroll
-        for (int x = 0; x < 32; x += 4) {
-          const float4 mu = *reinterpret_cast<const float4*>(mul + c + x), ad = *reinterpret_cast<const float4*>(add + c + x);
-          float4 in = *reinterpret_cast<const float4*>(inv + c + x);
-          float2 t0 = fma2(make_float2(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), make_float2(mu.x, mu.y), make_float2(ad.x, ad.y));
-          float2 t1 = fma2(make_float2(__uint_as_float(s[x + 2]), __uint_as_float(s[x + 3])), make_float2(mu.z, mu.w), make_float2(ad.z, ad.w));
-          if (partial) {
-            const int k = key0 + c + x;
-            if (k >= limit) t0.x = -INFINITY, in.x = 0.0f;
-            if (k + 1 >= limit) t0.y = -INFINITY, in.y = 0.0f;
-            if (k + 2 >= limit) t1.x = -INFINITY, in.z = 0.0f;
-            if (k + 3 >= limit) t1.y = -INFINITY, in.w = 0.0f;
-          }
-          t0 = add2(t0, base2);
-          t1 = add2(t1, base2);
-          t0 = make_float2(ex2(t0.x), ex2(t0.y));
-          t1 = make_float2(ex2(t1.x), ex2(t1.y));
-          l2 = fma2(t0, make_float2(in.x, in.y), l2);
-          l2 = fma2(t1, make_float2(in.z, in.w), l2);
-          p[x / 2] = pack_f16(t0.x, t0.y);
-          p[x / 2 + 1] = pack_f16(t1.x, t1.y);
-        }
-        tmem_store16(s_addr + c / 2, p);  // over columns of S that are already read
-      }
+      // over columns of S, all of which have been read
+      l2 = partial ? weigh<true>(t, base, inv, s_addr, l2) : weigh<false>(t, base, inv, s_addr, l2);
       tmem_wait_store();
       fence_before();
       bar_arrive(smem_u32(&sm.p_full[slot]));
@@ -308,59 +341,63 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
     }
   } else if (warp < 12) {
     // -------------------------------------------------------------- loading
+    // K's registers are loaded for the next tile while V is widened, and V's
+    // while the next K is; the page two tiles ahead is known by then.
+    registers_down<88>();
     const int lw = warp - 8;
     constexpr int KN = D / 16, VN = D / 32;
     uint4 kr[KN];
     uint4 vr[VN][2];
-    float ks = 0.0f, vs = 0.0f;
-    bool page_ok = false;
-    auto fetch = [&](int j) {
-      const int key0 = k0 + j * WIDE_KEYS + lw * 32;  // 32 keys of one page
-      page_ok = false;
-      if (key0 < k1) {
-        const uint32_t page = pages[key0 / KV_PAGE];
-        if (page < a.c.pages) {
-          page_ok = true;
-          const size_t block = (size_t)page * a.c.kv_heads + h;
-          const int in_page = key0 % KV_PAGE;
-          const uint8_t* kp = a.c.k + block * (KV_PAGE * D) + in_page * 64;
-          const uint8_t* vp = a.c.v + block * (KV_PAGE * D) + in_page * D;
-          // 8 keys x 4 pieces of 16 codes a load
+    float ks = 1.0f, vs = 1.0f;
+    auto page_of = [&](int j) -> uint32_t {  // of this warp's 32 keys of tile j
+      const int key0 = k0 + j * WIDE_KEYS + lw * 32;
+      return j < tiles && key0 < k1 ? pages[key0 / KV_PAGE] : 0xffffffffu;
+    };
+    auto fetch_k = [&](int j, uint32_t page) {
+      if (page < a.c.pages) {
+        const size_t block = (size_t)page * a.c.kv_heads + h;
+        const int in_page = (k0 + j * WIDE_KEYS + lw * 32) % KV_PAGE;
+        const uint8_t* kp = a.c.k + block * (KV_PAGE * D) + in_page * 64 + (lane & 7) * 64 + (lane >> 3) * 16;
+        // 8 keys x 4 pieces of 16 codes a load
 #pragma unroll
-          for (int x = 0; x < KN; ++x)
-            kr[x] = *reinterpret_cast<const uint4*>(kp + (x % (D / 64)) * (KV_PAGE * 64) + ((x / (D / 64)) * 8 + (lane & 7)) * 64 + (lane >> 3) * 16);
-          // two blocks of 16 keys; of each, eight keys of dimension groups 8t + lane % 8
-#pragma unroll
-          for (int x = 0; x < VN; ++x) {
-            const uint8_t* p = vp + (lane >> 4) * 16 * D + x * 512 + (lane & 7) * 64 + ((lane >> 3) & 1) * 32;
-            vr[x][0] = *reinterpret_cast<const uint4*>(p);
-            vr[x][1] = *reinterpret_cast<const uint4*>(p + 16);
-          }
-          ks = a.c.ks[block * KV_PAGE + in_page + lane];
-          vs = a.c.vs[block * KV_PAGE + in_page + lane];
-        } else if (lane == 0) {
-          atomicOr(a.c.error, KV_BAD_PAGE);
-        }
-      }
-      if (!page_ok) {
+        for (int x = 0; x < KN; ++x) kr[x] = *reinterpret_cast<const uint4*>(kp + (x % (D / 64)) * (KV_PAGE * 64) + (x / (D / 64)) * 8 * 64);
+        ks = a.c.ks[block * KV_PAGE + in_page + lane];
+        vs = a.c.vs[block * KV_PAGE + in_page + lane];
+      } else {
 #pragma unroll
         for (int x = 0; x < KN; ++x) kr[x] = make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto fetch_v = [&](int j, uint32_t page) {
+      if (page < a.c.pages) {
+        const size_t block = (size_t)page * a.c.kv_heads + h;
+        const int in_page = (k0 + j * WIDE_KEYS + lw * 32) % KV_PAGE;
+        // two blocks of 16 keys; of each, eight keys of dimension groups 8t + lane % 8
+        const uint8_t* p = a.c.v + block * (KV_PAGE * D) + in_page * D + (lane >> 4) * 16 * D + (lane & 7) * 64 + ((lane >> 3) & 1) * 32;
+#pragma unroll
+        for (int x = 0; x < VN; ++x) {
+          vr[x][0] = *reinterpret_cast<const uint4*>(p + x * 512);
+          vr[x][1] = *reinterpret_cast<const uint4*>(p + x * 512 + 16);
+        }
+      } else {
 #pragma unroll
         for (int x = 0; x < VN; ++x) vr[x][0] = vr[x][1] = make_uint4(0, 0, 0, 0);
       }
     };
-    if (tiles > 0) fetch(0);
+    uint32_t page = page_of(0), next = page_of(1);
+    fetch_k(0, page);
+    fetch_v(0, page);
     for (int j = 0; j < tiles && ok; ++j) {
       const int stage = j & 1;
+      const uint32_t after = page_of(j + 2);
+      const int key = lw * 32 + lane;
+      if (page >= a.c.pages && lane == 0 && k0 + j * WIDE_KEYS + lw * 32 < k1) atomicOr(a.c.error, KV_BAD_PAGE);
       if (j >= 2) ok = wait(smem_u32(&sm.k_empty[stage]), ((j >> 1) - 1) & 1);
       if (!ok) break;
-      {
-        const int key = lw * 32 + lane;
-        const bool seen = page_ok && k0 + j * WIDE_KEYS + key < k1;
-        sm.mul[j & 3][key] = seen ? __fmul_rn(ks, a.scale) : 0.0f;
-        sm.add[j & 3][key] = seen ? lg2(vs) : -INFINITY;
-        sm.inv[j & 3][key] = seen ? __frcp_rn(vs) : 0.0f;
-      }
+      const bool seen = page < a.c.pages && k0 + j * WIDE_KEYS + key < k1;
+      sm.mul[j & 3][key] = seen ? __fmul_rn(ks, a.scale) : 0.0f;
+      sm.add[j & 3][key] = seen ? lg2(vs) : -INFINITY;
+      sm.inv[j & 3][key] = seen ? __frcp_rn(vs) : 0.0f;
 #pragma unroll
       for (int x = 0; x < KN; ++x) {
         const uint32_t w[4] = {kr[x].x, kr[x].y, kr[x].z, kr[x].w};
@@ -373,6 +410,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       bar_arrive(smem_u32(&sm.k_full[stage]));
+      fetch_k(j + 1, next);
       if (j >= 2) ok = wait(smem_u32(&sm.v_empty[stage]), ((j >> 1) - 1) & 1);
       if (!ok) break;
 #pragma unroll
@@ -387,11 +425,14 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       bar_arrive(smem_u32(&sm.v_full[stage]));
-      if (j + 1 < tiles) fetch(j + 1);
+      fetch_v(j + 1, next);
+      page = next;
+      next = after;
     }
     if (!ok) sm.failed = 1;
   } else {
-    if (lane == 0 && events > 0) {
+    registers_down<40>();
+    if (warp == 12 && lane == 0 && events > 0) {
       // ------------------------------------------------ the matrix instructions
       const uint32_t q_addr = smem_u32(sm.q[0]);
       auto scores = [&](int e) {
