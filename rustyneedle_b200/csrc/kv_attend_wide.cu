@@ -13,6 +13,17 @@
 // memory, one lane of warp 12 issues the matrix instructions:
 //   S = Q K^T   Q and K codes (f16 or bf16) from shared memory, f32 in TMEM
 //   O += P V    P (f16) from TMEM, over the first half of S; V codes (f16)
+// Two modes, chosen by each CTA from the value scales of its own keys:
+//   plain  their ratio is at most 2^PLAIN_BITS: the values enter the product as
+//          f16(code · scale / R), R the power of two above the largest scale
+//          (2^-12 relative, no subnormals), the weights are the softmax's own,
+//          and a key costs the softmax one number, its scale
+//   exact  otherwise (and for NaN scales): the codes enter as they are and the
+//          value scales through the exponents, as in the 16-row kernel
+// A number for each key costs every row's thread 4 bytes of shared-memory
+// bandwidth, 1024 of a tile pair's 2048 tensor cycles at D = 128: three of
+// them made a tile pair 7000 cycles long, one 4000.
+//
 // O is rescaled in TMEM only when a row's maximum has grown by more than
 // SLACK: until then the weights just get larger, up to 2^(HEADROOM + SLACK).
 //
@@ -91,7 +102,7 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t phase) { return mbar_wait_polls(bar, phase, 1u << 18); }
 
 // The launch's 512 threads hold 128 registers each; the four warpgroups share
-// them out anew as 192 + 192 + 88 + 40 = 4 x 128.
+// them out anew as 184 + 184 + 104 + 40 = 4 x 128.
 template <int N>
 __device__ __forceinline__ void registers_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -101,21 +112,22 @@ __device__ __forceinline__ void registers_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// One row's 128 scores t (already scaled, the value scale's logarithm added)
-// to weights 2^(t + base): packed as f16 for the product, summed over inv.
-// PARTIAL: scores of -inf are keys that the row does not see, whose inv may be
-// anything.
-template <bool PARTIAL>
-__device__ __forceinline__ float2 weigh(const float2 (&t)[64], float base, const float* inv, uint32_t p_addr, float2 sum) {
+// One row's 128 scores t to weights 2^(t + base): packed as f16 for the
+// product and summed, in the exact mode over inv. PARTIAL: scores of -inf are
+// keys that the row does not see, whose inv may be anything.
+template <bool PLAIN, bool PARTIAL>
+__device__ __forceinline__ float weigh(const float2 (&t)[64], float base, const float* inv, uint32_t p_addr) {
   const float2 base2 = make_float2(base, base);
+  float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     uint32_t p[16];
 #pragma unroll
     for (int x = 0; x < 16; x += 2) {
-      float4 in = *reinterpret_cast<const float4*>(inv + c * 32 + x * 2);
       float2 w0 = t[c * 16 + x], w1 = t[c * 16 + x + 1];
-      if (PARTIAL) {
+      float4 in = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+      if (!PLAIN) in = *reinterpret_cast<const float4*>(inv + c * 32 + x * 2);
+      if (!PLAIN && PARTIAL) {
         in.x = w0.x == -INFINITY ? 0.0f : in.x;
         in.y = w0.y == -INFINITY ? 0.0f : in.y;
         in.z = w1.x == -INFINITY ? 0.0f : in.z;
@@ -125,15 +137,22 @@ __device__ __forceinline__ float2 weigh(const float2 (&t)[64], float base, const
       w1 = add2(w1, base2);
       w0 = make_float2(ex2(w0.x), ex2(w0.y));
       w1 = make_float2(ex2(w1.x), ex2(w1.y));
-      sum = fma2(w0, make_float2(in.x, in.y), sum);
-      sum = fma2(w1, make_float2(in.z, in.w), sum);
+      if (PLAIN) {
+        sum0 = add2(sum0, w0);
+        sum1 = add2(sum1, w1);
+      } else {
+        sum0 = fma2(w0, make_float2(in.x, in.y), sum0);
+        sum1 = fma2(w1, make_float2(in.z, in.w), sum1);
+      }
       p[x] = pack_f16(w0.x, w0.y);
       p[x + 1] = pack_f16(w1.x, w1.y);
     }
     tmem_store16(p_addr + c * 16, p);
   }
-  return sum;
+  return __fadd_rn(__fadd_rn(sum0.x, sum1.x), __fadd_rn(sum0.y, sum1.y));
 }
+
+constexpr int PLAIN_BITS = 12;
 
 template <int D>
 struct WideSmem {
@@ -146,6 +165,7 @@ struct WideSmem {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done;
   uint32_t tmem;
   int failed;
+  float scale_most[16], scale_least[16];
 };
 
 // grid (row tiles (or pairs) x sequences, kv heads, chunks), block 512
@@ -225,16 +245,40 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
     const int t = i & (WIDE_ROWS - 1);
     *reinterpret_cast<uint4*>(sm.q[i / WIDE_ROWS] + (t / 8) * ROW_SBO + chunk * 128 + (t % 8) * 16) = w;
   }
+  // the value scales of all keys, a half page a warp at once
+  float most = 0.0f, least = INFINITY;
+  for (int key0 = k0 + warp * 32; key0 < k1; key0 += WIDE_ATT_THREADS) {
+    const uint32_t page = pages[key0 / KV_PAGE];
+    if (page >= a.c.pages) {
+      least = -1.0f;  // its keys are masked one by one
+    } else if (key0 + lane < k1) {
+      const float vs = a.c.vs[((size_t)page * a.c.kv_heads + h) * KV_PAGE + key0 % KV_PAGE + lane];
+      most = fmaxf(most, vs);
+      least = vs == vs ? fminf(least, vs) : -1.0f;  // a NaN
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    most = fmaxf(most, __shfl_xor_sync(FULL, most, o));
+    least = fminf(least, __shfl_xor_sync(FULL, least, o));
+  }
+  if (lane == 0) sm.scale_most[warp] = most, sm.scale_least[warp] = least;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = sm.tmem;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) most = fmaxf(most, sm.scale_most[w]), least = fminf(least, sm.scale_least[w]);
+  const bool plain = least >= __fmul_rn(most, 1.0f / (1 << PLAIN_BITS)) && most > 0.0f;
+  // the power of two at or above the largest scale, and its reciprocal (scales lie in [2^-60, 2^34])
+  const float unit = plain ? __uint_as_float((__float_as_uint(most) + 0x7fffffu) & 0x7f800000u) : 1.0f;
+  const float per_unit = __uint_as_float(0x7f000000u - __float_as_uint(unit));
 
   bool ok = true;
   if (warp < 8) {
     // ------------------------------------------------------------- softmax
-    registers_up<192>();
+    registers_up<184>();
     const int slot = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + slot * 128, o_addr = tmem + lanes + 256 + slot * 128;
@@ -243,7 +287,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
     // keys below it are seen by every row of the warp
     const int all_see = prefix ? k1 : min(k1, sees0 + min(r - lane, rows - 1) / a.group + 1);
     float m = -INFINITY;
-    float2 l2 = make_float2(0.0f, 0.0f);
+    float l = 0.0f;
     int n = 0;
     for (int e = slot; e < events && ok; e += 2, ++n) {
       const int j = pair ? e >> 1 : e, key0 = k0 + j * WIDE_KEYS;
@@ -253,7 +297,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
       const float* mul = sm.mul[j & 3];
       const float* add = sm.add[j & 3];
       const float* inv = sm.inv[j & 3];
-      const bool partial = key0 + WIDE_KEYS > all_see && !prefix;
+      const bool partial = key0 + WIDE_KEYS > all_see;
       float2 t[64];
       {
         uint32_t r0[32], r1[32], r2[32], r3[32];
@@ -271,11 +315,21 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
         }
       }
       float top0 = -INFINITY, top1 = -INFINITY;
+      if (plain) {
+        const float2 zero = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int x = 0; x < 64; x += 2) {
-        const float4 mu = *reinterpret_cast<const float4*>(mul + 2 * x), ad = *reinterpret_cast<const float4*>(add + 2 * x);
-        t[x] = fma2(t[x], make_float2(mu.x, mu.y), make_float2(ad.x, ad.y));
-        t[x + 1] = fma2(t[x + 1], make_float2(mu.z, mu.w), make_float2(ad.z, ad.w));
+        for (int x = 0; x < 64; x += 2) {
+          const float4 mu = *reinterpret_cast<const float4*>(mul + 2 * x);
+          t[x] = fma2(t[x], make_float2(mu.x, mu.y), zero);
+          t[x + 1] = fma2(t[x + 1], make_float2(mu.z, mu.w), zero);
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 64; x += 2) {
+          const float4 mu = *reinterpret_cast<const float4*>(mul + 2 * x), ad = *reinterpret_cast<const float4*>(add + 2 * x);
+          t[x] = fma2(t[x], make_float2(mu.x, mu.y), make_float2(ad.x, ad.y));
+          t[x + 1] = fma2(t[x + 1], make_float2(mu.z, mu.w), make_float2(ad.z, ad.w));
+        }
       }
       if (partial) {
 #pragma unroll
@@ -295,7 +349,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
         const float next = grown ? fmaxf(m, want) : m;
         const float keep = next == m ? 1.0f : ex2(__fadd_rn(m, -next));
         m = next;
-        l2 = make_float2(__fmul_rn(l2.x, keep), __fmul_rn(l2.y, keep));
+        l = __fmul_rn(l, keep);
         if (n > 0) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -310,7 +364,12 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
       }
       const float base = m == -INFINITY ? 0.0f : -m;
       // over columns of S, all of which have been read
-      l2 = partial ? weigh<true>(t, base, inv, s_addr, l2) : weigh<false>(t, base, inv, s_addr, l2);
+      float sum;
+      if (plain)
+        sum = weigh<true, false>(t, base, inv, s_addr);
+      else
+        sum = partial ? weigh<false, true>(t, base, inv, s_addr) : weigh<false, false>(t, base, inv, s_addr);
+      l = __fadd_rn(l, sum);
       tmem_wait_store();
       fence_before();
       bar_arrive(smem_u32(&sm.p_full[slot]));
@@ -322,7 +381,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
     if (ok) {
       const int index = parts0 + (pair ? part : 2 * part + slot);
       const size_t at = r < rows ? ((size_t)index * a.b.rows + token0 + r / a.group) * a.heads + h * a.group + r % a.group : 0;
-      if (r < rows) a.part_ml[at] = make_float2(m, __fadd_rn(l2.x, l2.y));
+      if (r < rows) a.part_ml[at] = make_float2(m, l);
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -335,7 +394,8 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
         }
         if (r < rows) {
 #pragma unroll
-          for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(a.part_o + at * D + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+          for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(a.part_o + at * D + c + x) = make_uint4(__float_as_uint(__fmul_rn(__uint_as_float(o[x]), unit)), __float_as_uint(__fmul_rn(__uint_as_float(o[x + 1]), unit)),
+                           __float_as_uint(__fmul_rn(__uint_as_float(o[x + 2]), unit)), __float_as_uint(__fmul_rn(__uint_as_float(o[x + 3]), unit)));
         }
       }
     }
@@ -343,7 +403,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
     // -------------------------------------------------------------- loading
     // K's registers are loaded for the next tile while V is widened, and V's
     // while the next K is; the page two tiles ahead is known by then.
-    registers_down<88>();
+    registers_down<104>();
     const int lw = warp - 8;
     constexpr int KN = D / 16, VN = D / 32;
     uint4 kr[KN];
@@ -368,6 +428,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
         for (int x = 0; x < KN; ++x) kr[x] = make_uint4(0, 0, 0, 0);
       }
     };
+    float vs8[8];  // the value scales of the lane's eight keys of V
     auto fetch_v = [&](int j, uint32_t page) {
       if (page < a.c.pages) {
         const size_t block = (size_t)page * a.c.kv_heads + h;
@@ -379,6 +440,9 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
           vr[x][0] = *reinterpret_cast<const uint4*>(p + x * 512);
           vr[x][1] = *reinterpret_cast<const uint4*>(p + x * 512 + 16);
         }
+        const float4* scales = reinterpret_cast<const float4*>(a.c.vs + block * KV_PAGE + in_page + (lane >> 3) * 8);
+        const float4 s0 = scales[0], s1 = scales[1];
+        vs8[0] = s0.x, vs8[1] = s0.y, vs8[2] = s0.z, vs8[3] = s0.w, vs8[4] = s1.x, vs8[5] = s1.y, vs8[6] = s1.z, vs8[7] = s1.w;
       } else {
 #pragma unroll
         for (int x = 0; x < VN; ++x) vr[x][0] = vr[x][1] = make_uint4(0, 0, 0, 0);
@@ -413,14 +477,33 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
       fetch_k(j + 1, next);
       if (j >= 2) ok = wait(smem_u32(&sm.v_empty[stage]), ((j >> 1) - 1) & 1);
       if (!ok) break;
+      // scale / R as the sum of two halves: code · (hi + lo), rounded once
+      __half2 hi[4], lo[4];
+      if (plain) {
+        const int first = k0 + j * WIDE_KEYS + lw * 32 + (lane >> 3) * 8;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float s0 = page < a.c.pages && first + 2 * x < k1 ? __fmul_rn(vs8[2 * x], per_unit) : 0.0f;
+          const float s1 = page < a.c.pages && first + 2 * x + 1 < k1 ? __fmul_rn(vs8[2 * x + 1], per_unit) : 0.0f;
+          hi[x] = __floats2half2_rn(s0, s1);
+          const float2 back = __half22float2(hi[x]);
+          lo[x] = __floats2half2_rn(__fadd_rn(s0, -back.x), __fadd_rn(s1, -back.y));
+        }
+      }
+      auto scaled = [&](uint32_t codes, int x) -> uint32_t {
+        if (!plain) return codes;
+        const __half2 c = *reinterpret_cast<const __half2*>(&codes);
+        const __half2 v = __hfma2(c, hi[x], __hmul2(c, lo[x]));
+        return *reinterpret_cast<const uint32_t*>(&v);
+      };
 #pragma unroll
       for (int x = 0; x < VN; ++x) {
         const uint32_t w0[4] = {vr[x][0].x, vr[x][0].y, vr[x][0].z, vr[x][0].w}, w1[4] = {vr[x][1].x, vr[x][1].y, vr[x][1].z, vr[x][1].w};
         uint8_t* dst = sm.v[stage] + (lw * 4 + (lane >> 4) * 2 + ((lane >> 3) & 1)) * 128 + (lane & 7) * 16;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const uint2 lo = widen<E4M3, false>(w0[t]), hi = widen<E4M3, false>(w1[t]);
-          *reinterpret_cast<uint4*>(dst + (x * 4 + t) * V_SBO) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          const uint2 c0 = widen<E4M3, false>(w0[t]), c1 = widen<E4M3, false>(w1[t]);
+          *reinterpret_cast<uint4*>(dst + (x * 4 + t) * V_SBO) = make_uint4(scaled(c0.x, 0), scaled(c0.y, 1), scaled(c1.x, 2), scaled(c1.y, 3));
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
