@@ -7,22 +7,19 @@
 //              8-bit codes are widened once for 256 rows;
 //   one tile:  the slots are one row tile over alternate key tiles.
 // While one slot's scores go through the softmax, the tensor cores work for
-// the other. Warps 0-3 and 4-7 are the slots' softmax (a thread is a row:
-// TMEM lane = row; a row of 128 scores stays in registers between its maximum
-// and its exponentials), warps 8-11 load codes and widen them into shared
-// memory, one lane of warp 12 issues the matrix instructions:
+// the other. Warps 0-3 and 4-7 are the slots' softmax (a warp has 32 rows),
+// warps 8-11 load codes and widen them into shared memory, one lane of warp 12
+// issues the matrix instructions:
 //   S = Q K^T   Q and K codes (f16 or bf16) from shared memory, f32 in TMEM
 //   O += P V    P (f16) from TMEM, over the first half of S; V codes (f16)
-// Two modes, chosen by each CTA from the value scales of its own keys:
-//   plain  their ratio is at most 2^PLAIN_BITS: the values enter the product as
-//          f16(code · scale / R), R the power of two above the largest scale
-//          (2^-12 relative, no subnormals), the weights are the softmax's own,
-//          and a key costs the softmax one number, its scale
-//   exact  otherwise (and for NaN scales): the codes enter as they are and the
-//          value scales through the exponents, as in the 16-row kernel
-// A number for each key costs every row's thread 4 bytes of shared-memory
-// bandwidth, 1024 of a tile pair's 2048 tensor cycles at D = 128: three of
-// them made a tile pair 7000 cycles long, one 4000.
+//
+// The softmax reads TMEM in 16-lane pieces of 256 bits a row, so a thread has
+// 4 rows x 32 keys of the tile (rows lane / 4 + 8 k, keys 8 n + 2 (lane % 4)
+// and the next), not 1 x 128: a key's numbers (scale, the value scale's
+// logarithm and reciprocal) then serve 4 rows of a thread. Shared memory's 128
+// bytes a cycle are what is short here: for a tile pair at D = 128 the matrix
+// operands take 1536 cycles, the loaders' stores 512 and the keys' numbers 768;
+// with a row a thread they took 3072.
 //
 // O is rescaled in TMEM only when a row's maximum has grown by more than
 // SLACK: until then the weights just get larger, up to 2^(HEADROOM + SLACK).
@@ -67,31 +64,31 @@ __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
 
-__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
-      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
+// 128 columns of 16 lanes: registers 4 n, 4 n + 1 are row lane / 4, columns 8 n +
+// 2 (lane % 4) and the next; 4 n + 2, 4 n + 3 the same of row lane / 4 + 8.
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[64]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
-      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+// 32 columns of 16 lanes: registers 4 n, 4 n + 1 are row lane / 4, columns 8 n +
+// 2 (lane % 4) and the next; 4 n + 2, 4 n + 3 the same of row lane / 4 + 8.
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+// The inverse of the 32-column load.
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-      "r"(r[13]), "r"(r[14]), "r"(r[15])
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// 16 columns of 32 bits of 16 lanes: register 2 n is row lane / 4, column 4 n +
+// lane % 4, register 2 n + 1 the same of row lane / 4 + 8: pairs of f16 from the
+// 256-bit load's neighbouring columns.
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -102,7 +99,7 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t phase) { return mbar_wait_polls(bar, phase, 1u << 18); }
 
 // The launch's 512 threads hold 128 registers each; the four warpgroups share
-// them out anew as 184 + 184 + 104 + 40 = 4 x 128.
+// them out anew as 192 + 192 + 88 + 40 = 4 x 128.
 template <int N>
 __device__ __forceinline__ void registers_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -112,47 +109,39 @@ __device__ __forceinline__ void registers_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// One row's 128 scores t to weights 2^(t + base): packed as f16 for the
-// product and summed, in the exact mode over inv. PARTIAL: scores of -inf are
-// keys that the row does not see, whose inv may be anything.
-template <bool PLAIN, bool PARTIAL>
-__device__ __forceinline__ float weigh(const float2 (&t)[64], float base, const float* inv, uint32_t p_addr) {
-  const float2 base2 = make_float2(base, base);
-  float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
+// A thread's 4 x 32 scores to weights 2^(t + base): packed as f16 for the
+// product, over the columns of S, and summed over inv. PARTIAL: scores of -inf
+// are keys that the row does not see, whose inv may be anything.
+constexpr uint32_t HALF_LANES = 16u << 16;  // a warp's lanes 16 .. 31
+template <bool PARTIAL>
+__device__ __forceinline__ void weigh(const float2 (&t)[4][16], const float2 (&base)[4], const float* inv, uint32_t p_addr, float2 (&l)[4]) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t p[16];
+  for (int x0 = 0; x0 < 16; x0 += 4) {
+    uint32_t p[2][8];
 #pragma unroll
-    for (int x = 0; x < 16; x += 2) {
-      float2 w0 = t[c * 16 + x], w1 = t[c * 16 + x + 1];
-      float4 in = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-      if (!PLAIN) in = *reinterpret_cast<const float4*>(inv + c * 32 + x * 2);
-      if (!PLAIN && PARTIAL) {
-        in.x = w0.x == -INFINITY ? 0.0f : in.x;
-        in.y = w0.y == -INFINITY ? 0.0f : in.y;
-        in.z = w1.x == -INFINITY ? 0.0f : in.z;
-        in.w = w1.y == -INFINITY ? 0.0f : in.w;
+    for (int x = 0; x < 4; ++x) {
+      const float2 in = *reinterpret_cast<const float2*>(inv + 8 * (x0 + x));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 y = t[k][x0 + x];
+        float2 own = in;
+        if (PARTIAL) own = make_float2(y.x == -INFINITY ? 0.0f : in.x, y.y == -INFINITY ? 0.0f : in.y);
+        float2 w = add2(y, base[k]);
+        w = make_float2(ex2(w.x), ex2(w.y));
+        l[k] = fma2(w, own, l[k]);
+        p[k >> 1][2 * x + (k & 1)] = pack_f16(w.x, w.y);
       }
-      w0 = add2(w0, base2);
-      w1 = add2(w1, base2);
-      w0 = make_float2(ex2(w0.x), ex2(w0.y));
-      w1 = make_float2(ex2(w1.x), ex2(w1.y));
-      if (PLAIN) {
-        sum0 = add2(sum0, w0);
-        sum1 = add2(sum1, w1);
-      } else {
-        sum0 = fma2(w0, make_float2(in.x, in.y), sum0);
-        sum1 = fma2(w1, make_float2(in.z, in.w), sum1);
-      }
-      p[x] = pack_f16(w0.x, w0.y);
-      p[x + 1] = pack_f16(w1.x, w1.y);
     }
-    tmem_store16(p_addr + c * 16, p);
+    tmem_store(p_addr + x0 * 4, p[0]);
+    tmem_store(p_addr + HALF_LANES + x0 * 4, p[1]);
   }
-  return __fadd_rn(__fadd_rn(sum0.x, sum1.x), __fadd_rn(sum0.y, sum1.y));
 }
 
-constexpr int PLAIN_BITS = 12;
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 template <int D>
 struct WideSmem {
@@ -165,7 +154,6 @@ struct WideSmem {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done;
   uint32_t tmem;
   int failed;
-  float scale_most[16], scale_least[16];
 };
 
 // grid (row tiles (or pairs) x sequences, kv heads, chunks), block 512
@@ -245,131 +233,106 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
     const int t = i & (WIDE_ROWS - 1);
     *reinterpret_cast<uint4*>(sm.q[i / WIDE_ROWS] + (t / 8) * ROW_SBO + chunk * 128 + (t % 8) * 16) = w;
   }
-  // the value scales of all keys, a half page a warp at once
-  float most = 0.0f, least = INFINITY;
-  for (int key0 = k0 + warp * 32; key0 < k1; key0 += WIDE_ATT_THREADS) {
-    const uint32_t page = pages[key0 / KV_PAGE];
-    if (page >= a.c.pages) {
-      least = -1.0f;  // its keys are masked one by one
-    } else if (key0 + lane < k1) {
-      const float vs = a.c.vs[((size_t)page * a.c.kv_heads + h) * KV_PAGE + key0 % KV_PAGE + lane];
-      most = fmaxf(most, vs);
-      least = vs == vs ? fminf(least, vs) : -1.0f;  // a NaN
-    }
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    most = fmaxf(most, __shfl_xor_sync(FULL, most, o));
-    least = fminf(least, __shfl_xor_sync(FULL, least, o));
-  }
-  if (lane == 0) sm.scale_most[warp] = most, sm.scale_least[warp] = least;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = sm.tmem;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) most = fmaxf(most, sm.scale_most[w]), least = fminf(least, sm.scale_least[w]);
-  const bool plain = least >= __fmul_rn(most, 1.0f / (1 << PLAIN_BITS)) && most > 0.0f;
-  // the power of two at or above the largest scale, and its reciprocal (scales lie in [2^-60, 2^34])
-  const float unit = plain ? __uint_as_float((__float_as_uint(most) + 0x7fffffu) & 0x7f800000u) : 1.0f;
-  const float per_unit = __uint_as_float(0x7f000000u - __float_as_uint(unit));
 
   bool ok = true;
   if (warp < 8) {
     // ------------------------------------------------------------- softmax
-    registers_up<184>();
-    const int slot = warp >> 2;
+    registers_up<192>();
+    const int slot = warp >> 2, g = lane >> 2, c2 = (lane & 3) * 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + slot * 128, o_addr = tmem + lanes + 256 + slot * 128;
-    const int i = (pair ? slot * WIDE_ROWS : 0) + (warp & 3) * 32 + lane, r = row0 + i;
-    const int limit = prefix ? k1 : min(k1, sees0 + min(r, rows - 1) / a.group + 1);
+    // the thread's rows: first + 8 k
+    const int first = row0 + (pair ? slot * WIDE_ROWS : 0) + (warp & 3) * 32 + g;
+    int limit[4];  // keys below it are seen by row k
+#pragma unroll
+    for (int k = 0; k < 4; ++k) limit[k] = prefix ? k1 : min(k1, sees0 + min(first + 8 * k, rows - 1) / a.group + 1);
     // keys below it are seen by every row of the warp
-    const int all_see = prefix ? k1 : min(k1, sees0 + min(r - lane, rows - 1) / a.group + 1);
-    float m = -INFINITY;
-    float l = 0.0f;
+    const int all_see = prefix ? k1 : min(k1, sees0 + min(first - g, rows - 1) / a.group + 1);
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    float2 l[4] = {};
     int n = 0;
     for (int e = slot; e < events && ok; e += 2, ++n) {
       const int j = pair ? e >> 1 : e, key0 = k0 + j * WIDE_KEYS;
       ok = __all_sync(FULL, wait(smem_u32(&sm.s_full[slot]), n & 1));
       if (!ok) break;
       fence_after();
-      const float* mul = sm.mul[j & 3];
-      const float* add = sm.add[j & 3];
-      const float* inv = sm.inv[j & 3];
-      const bool partial = key0 + WIDE_KEYS > all_see;
-      float2 t[64];
+      const float* mul = sm.mul[j & 3] + c2;
+      const float* add = sm.add[j & 3] + c2;
+      const float* inv = sm.inv[j & 3] + c2;
+      float2 t[4][16];
       {
-        uint32_t r0[32], r1[32], r2[32], r3[32];
-        tmem_load32(s_addr, r0);
-        tmem_load32(s_addr + 32, r1);
-        tmem_load32(s_addr + 64, r2);
-        tmem_load32(s_addr + 96, r3);
+        uint32_t lo[64], hi[64];
+        tmem_load(s_addr, lo);
+        tmem_load(s_addr + HALF_LANES, hi);
         tmem_wait_load();
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-          t[x] = make_float2(__uint_as_float(r0[2 * x]), __uint_as_float(r0[2 * x + 1]));
-          t[16 + x] = make_float2(__uint_as_float(r1[2 * x]), __uint_as_float(r1[2 * x + 1]));
-          t[32 + x] = make_float2(__uint_as_float(r2[2 * x]), __uint_as_float(r2[2 * x + 1]));
-          t[48 + x] = make_float2(__uint_as_float(r3[2 * x]), __uint_as_float(r3[2 * x + 1]));
+          const float2 mu = *reinterpret_cast<const float2*>(mul + 8 * x), ad = *reinterpret_cast<const float2*>(add + 8 * x);
+          t[0][x] = fma2(make_float2(__uint_as_float(lo[4 * x]), __uint_as_float(lo[4 * x + 1])), mu, ad);
+          t[1][x] = fma2(make_float2(__uint_as_float(lo[4 * x + 2]), __uint_as_float(lo[4 * x + 3])), mu, ad);
+          t[2][x] = fma2(make_float2(__uint_as_float(hi[4 * x]), __uint_as_float(hi[4 * x + 1])), mu, ad);
+          t[3][x] = fma2(make_float2(__uint_as_float(hi[4 * x + 2]), __uint_as_float(hi[4 * x + 3])), mu, ad);
         }
       }
-      float top0 = -INFINITY, top1 = -INFINITY;
-      if (plain) {
-        const float2 zero = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int x = 0; x < 64; x += 2) {
-          const float4 mu = *reinterpret_cast<const float4*>(mul + 2 * x);
-          t[x] = fma2(t[x], make_float2(mu.x, mu.y), zero);
-          t[x + 1] = fma2(t[x + 1], make_float2(mu.z, mu.w), zero);
-        }
-      } else {
-#pragma unroll
-        for (int x = 0; x < 64; x += 2) {
-          const float4 mu = *reinterpret_cast<const float4*>(mul + 2 * x), ad = *reinterpret_cast<const float4*>(add + 2 * x);
-          t[x] = fma2(t[x], make_float2(mu.x, mu.y), make_float2(ad.x, ad.y));
-          t[x + 1] = fma2(t[x + 1], make_float2(mu.z, mu.w), make_float2(ad.z, ad.w));
-        }
-      }
+      const bool partial = key0 + WIDE_KEYS > all_see && !prefix;
       if (partial) {
 #pragma unroll
-        for (int x = 0; x < 64; ++x) {
-          t[x].x = key0 + 2 * x < limit ? t[x].x : -INFINITY;
-          t[x].y = key0 + 2 * x + 1 < limit ? t[x].y : -INFINITY;
-        }
-      }
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int x = 0; x < 64; x += 2) {
-        top0 = fmaxf(top0, fmaxf(t[x].x, t[x].y));
-        top1 = fmaxf(top1, fmaxf(t[x + 1].x, t[x + 1].y));
+          for (int x = 0; x < 16; ++x) {
+            t[k][x].x = key0 + 8 * x + c2 < limit[k] ? t[k][x].x : -INFINITY;
+            t[k][x].y = key0 + 8 * x + c2 + 1 < limit[k] ? t[k][x].y : -INFINITY;
+          }
       }
-      const float want = __fadd_rn(fmaxf(top0, top1), -HEADROOM);
-      const bool grown = want > __fadd_rn(m, SLACK) || m == -INFINITY;
+      float want[4];
+      bool grown = false;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float top = fmaxf(t[k][0].x, t[k][0].y);
+#pragma unroll
+        for (int x = 1; x < 16; ++x) top = max3(top, t[k][x].x, t[k][x].y);
+        top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+        want[k] = __fadd_rn(top, -HEADROOM);
+        grown = grown || want[k] > __fadd_rn(m[k], SLACK) || (m[k] == -INFINITY && want[k] != -INFINITY);
+      }
       if (__any_sync(FULL, grown)) {
-        const float next = grown ? fmaxf(m, want) : m;
-        const float keep = next == m ? 1.0f : ex2(__fadd_rn(m, -next));
-        m = next;
-        l = __fmul_rn(l, keep);
+        float keep[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float next = fmaxf(m[k], want[k]);
+          keep[k] = next == m[k] ? 1.0f : ex2(__fadd_rn(m[k], -next));
+          m[k] = next;
+          l[k] = make_float2(__fmul_rn(l[k].x, keep[k]), __fmul_rn(l[k].y, keep[k]));
+        }
         if (n > 0) {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_load32(o_addr + c, o);
+          for (int c = 0; c < 2 * D; c += 32) {  // both halves of the lanes
+            const uint32_t at = o_addr + (c % D) + (c < D ? 0u : HALF_LANES);
+            const float low = c < D ? keep[0] : keep[2], high = c < D ? keep[1] : keep[3];
+            uint32_t o[16];
+            tmem_load(at, o);
             tmem_wait_load();
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__fmul_rn(__uint_as_float(o[x]), keep));
-            tmem_store32(o_addr + c, o);
+            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__fmul_rn(__uint_as_float(o[x]), x & 2 ? high : low));
+            tmem_store(at, o);
           }
         }
       }
-      const float base = m == -INFINITY ? 0.0f : -m;
-      // over columns of S, all of which have been read
-      float sum;
-      if (plain)
-        sum = weigh<true, false>(t, base, inv, s_addr);
+      // weights 2^(t - m): packed as f16 for the product, over columns of S (all
+      // of which have been read), and summed over inv
+      float2 base[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) base[k].x = base[k].y = m[k] == -INFINITY ? 0.0f : -m[k];
+      if (partial)
+        weigh<true>(t, base, inv, s_addr, l);
       else
-        sum = partial ? weigh<false, true>(t, base, inv, s_addr) : weigh<false, false>(t, base, inv, s_addr);
-      l = __fadd_rn(l, sum);
+        weigh<false>(t, base, inv, s_addr, l);
       tmem_wait_store();
       fence_before();
       bar_arrive(smem_u32(&sm.p_full[slot]));
@@ -377,33 +340,44 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
     if (!ok) sm.failed = 1;
     if (ok && tiles > 0) ok = __all_sync(FULL, wait(smem_u32(&sm.done), 0));
     fence_after();
-    // this row's part; a slot without a key tile of its own has sum 0
+    // the rows' part; a slot without a key tile of its own has sum 0
     if (ok) {
       const int index = parts0 + (pair ? part : 2 * part + slot);
-      const size_t at = r < rows ? ((size_t)index * a.b.rows + token0 + r / a.group) * a.heads + h * a.group + r % a.group : 0;
-      if (r < rows) a.part_ml[at] = make_float2(m, l);
+      size_t at[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = first + 8 * k;
+        at[k] = r < rows ? ((size_t)index * a.b.rows + token0 + r / a.group) * a.heads + h * a.group + r % a.group : 0;
+        float sum = __fadd_rn(l[k].x, l[k].y);
+        sum = __fadd_rn(sum, __shfl_xor_sync(FULL, sum, 1));
+        sum = __fadd_rn(sum, __shfl_xor_sync(FULL, sum, 2));
+        if (r < rows && c2 == 0) a.part_ml[at[k]] = make_float2(m[k], sum);
+      }
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
+        uint32_t o[2][16];
         if (n > 0) {
-          tmem_load32(o_addr + c, o);
+          tmem_load(o_addr + c, o[0]);
+          tmem_load(o_addr + HALF_LANES + c, o[1]);
           tmem_wait_load();
         } else {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) o[x] = 0u;
+          for (int x = 0; x < 16; ++x) o[0][x] = o[1][x] = 0u;
         }
-        if (r < rows) {
 #pragma unroll
-          for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(a.part_o + at * D + c + x) = make_uint4(__float_as_uint(__fmul_rn(__uint_as_float(o[x]), unit)), __float_as_uint(__fmul_rn(__uint_as_float(o[x + 1]), unit)),
-                           __float_as_uint(__fmul_rn(__uint_as_float(o[x + 2]), unit)), __float_as_uint(__fmul_rn(__uint_as_float(o[x + 3]), unit)));
-        }
+        for (int k = 0; k < 4; ++k)
+          if (first + 8 * k < rows) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              *reinterpret_cast<uint2*>(a.part_o + at[k] * D + c + 8 * x + c2) = make_uint2(o[k >> 1][4 * x + (k & 1) * 2], o[k >> 1][4 * x + (k & 1) * 2 + 1]);
+          }
       }
     }
   } else if (warp < 12) {
     // -------------------------------------------------------------- loading
     // K's registers are loaded for the next tile while V is widened, and V's
     // while the next K is; the page two tiles ahead is known by then.
-    registers_down<104>();
+    registers_down<88>();
     const int lw = warp - 8;
     constexpr int KN = D / 16, VN = D / 32;
     uint4 kr[KN];
@@ -428,7 +402,6 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
         for (int x = 0; x < KN; ++x) kr[x] = make_uint4(0, 0, 0, 0);
       }
     };
-    float vs8[8];  // the value scales of the lane's eight keys of V
     auto fetch_v = [&](int j, uint32_t page) {
       if (page < a.c.pages) {
         const size_t block = (size_t)page * a.c.kv_heads + h;
@@ -440,9 +413,6 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
           vr[x][0] = *reinterpret_cast<const uint4*>(p + x * 512);
           vr[x][1] = *reinterpret_cast<const uint4*>(p + x * 512 + 16);
         }
-        const float4* scales = reinterpret_cast<const float4*>(a.c.vs + block * KV_PAGE + in_page + (lane >> 3) * 8);
-        const float4 s0 = scales[0], s1 = scales[1];
-        vs8[0] = s0.x, vs8[1] = s0.y, vs8[2] = s0.z, vs8[3] = s0.w, vs8[4] = s1.x, vs8[5] = s1.y, vs8[6] = s1.z, vs8[7] = s1.w;
       } else {
 #pragma unroll
         for (int x = 0; x < VN; ++x) vr[x][0] = vr[x][1] = make_uint4(0, 0, 0, 0);
@@ -477,33 +447,14 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
       fetch_k(j + 1, next);
       if (j >= 2) ok = wait(smem_u32(&sm.v_empty[stage]), ((j >> 1) - 1) & 1);
       if (!ok) break;
-      // scale / R as the sum of two halves: code · (hi + lo), rounded once
-      __half2 hi[4], lo[4];
-      if (plain) {
-        const int first = k0 + j * WIDE_KEYS + lw * 32 + (lane >> 3) * 8;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float s0 = page < a.c.pages && first + 2 * x < k1 ? __fmul_rn(vs8[2 * x], per_unit) : 0.0f;
-          const float s1 = page < a.c.pages && first + 2 * x + 1 < k1 ? __fmul_rn(vs8[2 * x + 1], per_unit) : 0.0f;
-          hi[x] = __floats2half2_rn(s0, s1);
-          const float2 back = __half22float2(hi[x]);
-          lo[x] = __floats2half2_rn(__fadd_rn(s0, -back.x), __fadd_rn(s1, -back.y));
-        }
-      }
-      auto scaled = [&](uint32_t codes, int x) -> uint32_t {
-        if (!plain) return codes;
-        const __half2 c = *reinterpret_cast<const __half2*>(&codes);
-        const __half2 v = __hfma2(c, hi[x], __hmul2(c, lo[x]));
-        return *reinterpret_cast<const uint32_t*>(&v);
-      };
 #pragma unroll
       for (int x = 0; x < VN; ++x) {
         const uint32_t w0[4] = {vr[x][0].x, vr[x][0].y, vr[x][0].z, vr[x][0].w}, w1[4] = {vr[x][1].x, vr[x][1].y, vr[x][1].z, vr[x][1].w};
         uint8_t* dst = sm.v[stage] + (lw * 4 + (lane >> 4) * 2 + ((lane >> 3) & 1)) * 128 + (lane & 7) * 16;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const uint2 c0 = widen<E4M3, false>(w0[t]), c1 = widen<E4M3, false>(w1[t]);
-          *reinterpret_cast<uint4*>(dst + (x * 4 + t) * V_SBO) = make_uint4(scaled(c0.x, 0), scaled(c0.y, 1), scaled(c1.x, 2), scaled(c1.y, 3));
+          const uint2 lo = widen<E4M3, false>(w0[t]), hi = widen<E4M3, false>(w1[t]);
+          *reinterpret_cast<uint4*>(dst + (x * 4 + t) * V_SBO) = make_uint4(lo.x, lo.y, hi.x, hi.y);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

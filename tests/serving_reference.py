@@ -35,8 +35,7 @@ def e4m3(y):
 def attend(query, keys, codes, scales, rows, lengths, prefix, scale):
     """query [rows][heads][dim]; keys and the values' codes [prefix + sum(lengths)][kv][dim] and scales [..][kv]: the
     prefix's positions, then each sequence's. Returns the result and, for each of its elements, the sum of p |v|, the
-    largest sum of |q k| and the larger of: the largest p vs times the sum of the codes' sizes, the largest p times the sum
-    of the values' sizes."""
+    largest sum of |q k| and the largest p vs times the sum of the codes' sizes."""
     heads, dim = query.shape[1:]
     kv = keys.shape[1]
     out = np.zeros(query.shape)
@@ -60,7 +59,7 @@ def attend(query, keys, codes, scales, rows, lengths, prefix, scale):
                     p /= p.sum()
                     out[row + i, h] = p @ v
                     mass[row + i, h] = p @ np.abs(v)
-                    least[row + i, h] = np.maximum((p * scales[seen, j]).max() * np.abs(codes[seen, j]).sum(0), p.max() * np.abs(v).sum(0))
+                    least[row + i, h] = (p * scales[seen, j]).max() * np.abs(codes[seen, j]).sum(0)
                     size[row + i, h] = (np.abs(k) @ np.abs(q)).max() * abs(scale)
         row, at = row + r, at + t
     return out, mass, size, least

@@ -237,10 +237,7 @@ def check_attend(nb, torch, cache, query, keys, values, rows, lengths, table, pr
     The bound for one element, to first order:
       half a step of the output's type, relative: eps / 2
       the f16 rounding of each weight w: 2^-11 of sum p |v|; a weight below f16's normal numbers is off by 2^-25 at most, with
-        the largest weight (p vs with codes in the product, p with values there) at 2^8 or above: 2^-33 of the largest p vs (p),
-        times the code (the value), summed over the keys
-      where 33 and more rows meet the same keys, the values' own f16 rounding in the product (relative to the scale's power of
-        two; scales of such a launch differ by 2^12 at most, so no code of 1 and more is subnormal): once more 2^-11 of sum p |v|
+        the largest weight (p vs, scaled) at 2^8 or above: 2^-33 of the largest p vs, times the code, summed over the keys
       a score's f32 products and sums: dim + 8 roundings (2^-23 each) of sum |q k| scale, and exp2's and log2's own error, 2^-20;
         a weight's error enters the sum above and the one below it
       the f32 sums over the keys: 2^-23 for each of n / 8 products and 16 joins."""
@@ -256,7 +253,7 @@ def check_attend(nb, torch, cache, query, keys, values, rows, lengths, table, pr
     want, mass, size, least = ref.attend(numbers(query[:n]), kc * ks[..., None], vc, vs, rows, lengths, prefix, scale_)
     most = prefix + max(lengths, default=0)
     score = 2 * ((query.shape[2] + 8) * 2.0**-23 * size + 2.0**-20)
-    bound = torch.finfo(t).eps / 2 * np.abs(want) + mass * (2 * 2.0**-11 + score + (most / 8 + 16) * 2.0**-23) + 2.0**-33 * least + float(torch.finfo(t).smallest_normal) * 2.0**-8
+    bound = torch.finfo(t).eps / 2 * np.abs(want) + mass * (2.0**-11 + score + (most / 8 + 16) * 2.0**-23) + 2.0**-33 * least + float(torch.finfo(t).smallest_normal) * 2.0**-8
     got = numbers(result[:n])
     assert np.array_equal(np.isnan(got), np.isnan(want))
     off, bound = np.where(np.isnan(want), 0, np.abs(got - want)), np.where(np.isnan(want), 0, bound)  # NaN is compared above
