@@ -62,12 +62,6 @@ struct AttSmem {
   int failed;
 };
 
-__device__ __forceinline__ float rcp_fast(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 template <bool BF16>
 __device__ __forceinline__ void store_out4(const RowsDev& out, bool vector, long long at, const float (&y)[4]) {
   uint2 w;

@@ -42,19 +42,26 @@ __device__ __forceinline__ uint64_t core_desc(uint32_t addr, uint32_t sbo) {
   return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)((sbo >> 4) & 0x3fff) << 32) | (1ull << 46);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
+// The issuing warp runs as a whole, its operands the same in every lane (so
+// that they live in uniform registers: through one lane's vector registers an
+// event's instructions took 1850 cycles, three times their execution), and one
+// elected lane issues.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t leader;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+  return leader != 0;
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  if (accumulate)
+    asm volatile("tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, 1;" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+  else
+    asm volatile("tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, 0;" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  if (accumulate)
+    asm volatile("tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, 1;" ::"r"(d), "r"(a), "l"(b), "r"(idesc) : "memory");
+  else
+    asm volatile("tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, 0;" ::"r"(d), "r"(a), "l"(b), "r"(idesc) : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -466,42 +473,50 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
     if (!ok) sm.failed = 1;
   } else {
     registers_down<40>();
-    if (warp == 12 && lane == 0 && events > 0) {
+    if (warp == 12) {
       // ------------------------------------------------ the matrix instructions
-      const uint32_t q_addr = smem_u32(sm.q[0]);
+      // (all 512 columns are allocated: the TMEM address is 0)
+      constexpr uint64_t STAGE = WIDE_KEYS * D * 2 / 16;
+      const uint64_t q_desc = core_desc(smem_u32(sm.q[0]), ROW_SBO), k_desc = core_desc(smem_u32(sm.k[0]), ROW_SBO), v_desc = core_desc(smem_u32(sm.v[0]), V_SBO);
       auto scores = [&](int e) {
         const int slot = e & 1, j = pair ? e >> 1 : e, stage = j & 1;
         if (!pair || slot == 0) {
-          ok = ok && wait(smem_u32(&sm.k_full[stage]), (j >> 1) & 1);
+          ok = ok && __all_sync(FULL, wait(smem_u32(&sm.k_full[stage]), (j >> 1) & 1));
           fence_after();
         }
         if (!ok) return;
-        const uint32_t qa = q_addr + (pair ? slot * WIDE_ROWS * D * 2 : 0), ka = smem_u32(sm.k[stage]);
-  #pragma unroll
-        for (int x = 0; x < D / 16; ++x)
-          mma_ss(tmem + slot * 128, core_desc(qa + x * 256, ROW_SBO), core_desc(ka + x * 256, ROW_SBO), S_IDESC, x > 0);
-        mma_commit(smem_u32(&sm.s_full[slot]));
-        if (!pair || slot == 1) mma_commit(smem_u32(&sm.k_empty[stage]));
+        const uint64_t qa = q_desc + (pair ? slot * (WIDE_ROWS * D * 2 / 16) : 0), ka = k_desc + stage * STAGE;
+        if (elect_one()) {
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x) mma_ss(slot * 128, qa + x * 16, ka + x * 16, S_IDESC, x > 0);
+          mma_commit(smem_u32(&sm.s_full[slot]));
+          if (!pair || slot == 1) mma_commit(smem_u32(&sm.k_empty[stage]));
+        }
+        __syncwarp();
       };
-      scores(0);
-      if (events > 1) scores(1);
+      for (int e = 0; e < 2 && e < events; ++e) scores(e);
       for (int e = 0; e < events && ok; ++e) {
         const int slot = e & 1, j = pair ? e >> 1 : e, stage = j & 1;
-        ok = wait(smem_u32(&sm.p_full[slot]), (e >> 1) & 1);
-        if (ok && (!pair || slot == 0)) ok = wait(smem_u32(&sm.v_full[stage]), (j >> 1) & 1);
+        ok = __all_sync(FULL, wait(smem_u32(&sm.p_full[slot]), (e >> 1) & 1));
+        if (ok && (!pair || slot == 0)) ok = __all_sync(FULL, wait(smem_u32(&sm.v_full[stage]), (j >> 1) & 1));
         if (!ok) break;
         fence_after();
-        const uint32_t va = smem_u32(sm.v[stage]);
-  #pragma unroll
-        for (int x = 0; x < WIDE_KEYS / 16; ++x)
-          mma_ts(tmem + 256 + slot * 128, tmem + slot * 128 + x * 8, core_desc(va + x * 256, V_SBO), O_IDESC, e >= 2 || x > 0);
-        if (!pair || slot == 1) mma_commit(smem_u32(&sm.v_empty[stage]));
+        const uint64_t va = v_desc + stage * STAGE;
+        if (elect_one()) {
+#pragma unroll
+          for (int x = 0; x < WIDE_KEYS / 16; ++x) mma_ts(256 + slot * 128, slot * 128 + x * 8, va + x * 16, O_IDESC, e >= 2 || x > 0);
+          if (!pair || slot == 1) mma_commit(smem_u32(&sm.v_empty[stage]));
+        }
+        __syncwarp();
         if (e + 2 < events) scores(e + 2);
       }
-      mma_commit(smem_u32(&sm.done));
-      if (!ok) {
-        sm.failed = 1;
-        wait(smem_u32(&sm.done), 0);  // what was issued ends before the TMEM is freed
+      if (events > 0) {
+        if (elect_one()) mma_commit(smem_u32(&sm.done));
+        __syncwarp();
+        if (!ok) {
+          sm.failed = 1;
+          wait(smem_u32(&sm.done), 0);  // what was issued ends before the TMEM is freed
+        }
       }
     }
     __syncwarp();
