@@ -76,6 +76,8 @@ def numbers(t):
 CACHE_CASES = [  # rows of each sequence, positions before them
     ([1], [0]), ([1], [63]), ([1], [64]), ([3, 0, 5, 1], [0, 10, 62, 200]), ([130], [0]), ([65, 1, 17], [63, 64, 31]), ([0, 0], [5, 0]),
     ([2] * 70, list(range(70))), ([5, 16, 33, 48], [3, 16, 15, 1]),
+    # many rows: blocks of 16 rows with every alignment of their positions, across pages and sequences
+    ([2000 + i for i in range(6)], [0, 1, 2, 3, 17, 50]), ([7, 900, 0, 1, 4000, 33, 3500, 16], [5, 62, 3, 0, 6, 127, 1, 48]),
 ]
 
 
