@@ -33,7 +33,7 @@
 namespace nbk {
 
 constexpr int WIDE_ROWS = 128, WIDE_KEYS = 128, WIDE_ATT_THREADS = 16 * 32;
-constexpr int WIDE_LOADERS = 128;
+constexpr int WIDE_LOADERS = 4;  // warps
 constexpr float SLACK = 6.0f;
 
 // K-major operands without swizzle: 8 rows x 16 bytes make a core matrix of
@@ -66,7 +66,13 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// One arrival for a warp: 32 lanes' arrivals on one barrier are served one
+// after another, and with a few hundred of them a tile they were what took
+// the time.
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -217,7 +223,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
       bar_init(smem_u32(&sm.k_empty[i]), 1);
       bar_init(smem_u32(&sm.v_empty[i]), 1);
       bar_init(smem_u32(&sm.s_full[i]), 1);
-      bar_init(smem_u32(&sm.p_full[i]), WIDE_ROWS);
+      bar_init(smem_u32(&sm.p_full[i]), WIDE_ROWS / 32);
     }
     bar_init(smem_u32(&sm.done), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -342,7 +348,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
         weigh<false>(t, base, inv, s_addr, l);
       tmem_wait_store();
       fence_before();
-      bar_arrive(smem_u32(&sm.p_full[slot]));
+      warp_arrive(smem_u32(&sm.p_full[slot]));
     }
     if (!ok) sm.failed = 1;
     if (ok && tiles > 0) ok = __all_sync(FULL, wait(smem_u32(&sm.done), 0));
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
       const uint32_t after = page_of(j + 2);
       const int key = lw * 32 + lane;
       if (page >= a.c.pages && lane == 0 && k0 + j * WIDE_KEYS + lw * 32 < k1) atomicOr(a.c.error, KV_BAD_PAGE);
-      if (j >= 2) ok = wait(smem_u32(&sm.k_empty[stage]), ((j >> 1) - 1) & 1);
+      if (j >= 2) ok = __all_sync(FULL, wait(smem_u32(&sm.k_empty[stage]), ((j >> 1) - 1) & 1));
       if (!ok) break;
       const bool seen = page < a.c.pages && k0 + j * WIDE_KEYS + key < k1;
       sm.mul[j & 3][key] = seen ? __fmul_rn(ks, a.scale) : 0.0f;
@@ -450,9 +456,9 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(smem_u32(&sm.k_full[stage]));
+      warp_arrive(smem_u32(&sm.k_full[stage]));
       fetch_k(j + 1, next);
-      if (j >= 2) ok = wait(smem_u32(&sm.v_empty[stage]), ((j >> 1) - 1) & 1);
+      if (j >= 2) ok = __all_sync(FULL, wait(smem_u32(&sm.v_empty[stage]), ((j >> 1) - 1) & 1));
       if (!ok) break;
 #pragma unroll
       for (int x = 0; x < VN; ++x) {
@@ -465,7 +471,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(smem_u32(&sm.v_full[stage]));
+      warp_arrive(smem_u32(&sm.v_full[stage]));
       fetch_v(j + 1, next);
       page = next;
       next = after;
