@@ -9,6 +9,8 @@
 // softmax's own sum. m is the running maximum of t less HEADROOM, so w_j ≤
 // 2^HEADROOM; the product with the codes takes w as f16 (2^-12 relative down
 // to 2^-14, absolute 2^-25 below), the sums take it as f32.
+#include <cmath>
+
 #include "kv_attend.cuh"
 
 namespace nbk {
@@ -81,6 +83,52 @@ __device__ __forceinline__ void store_out4(const RowsDev& out, bool vector, long
     p[3] = (uint16_t)(w.y >> 16);
   }
 }
+
+// A row's running sum: y = Σ w code and sum = Σ w / vs under the maximum top.
+struct Joined {
+  float top = -INFINITY, sum = 0.0f, y[4] = {};
+
+  // four parts at a time, whose loads are in flight together
+  __device__ __forceinline__ void add(const float2 (&ml)[4], const float4 (&v)[4]) {
+    const float next = fmaxf(fmaxf(fmaxf(top, ml[0].x), fmaxf(ml[1].x, ml[2].x)), ml[3].x), base = next == -INFINITY ? 0.0f : next;
+    const float keep = ex2(__fadd_rn(top, -base));
+    top = next;
+    sum = __fmul_rn(sum, keep);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(y[e], keep);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = ex2(__fadd_rn(ml[i].x, -base));
+      sum = __fmaf_rn(ml[i].y, f, sum);
+      y[0] = __fmaf_rn(v[i].x, f, y[0]);
+      y[1] = __fmaf_rn(v[i].y, f, y[1]);
+      y[2] = __fmaf_rn(v[i].z, f, y[2]);
+      y[3] = __fmaf_rn(v[i].w, f, y[3]);
+    }
+  }
+  // the parts first, first + step .. of unit (token, head), dimensions d .. d + 3
+  template <int D>
+  __device__ __forceinline__ void add_parts(const AttendDev& a, size_t stride, size_t unit, int d, int first, int step, int parts) {
+    for (int p = first; p < parts; p += 4 * step) {
+      float2 ml[4];
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool some = p + i * step < parts;
+        const size_t at = (size_t)(p + i * step) * stride + unit;
+        ml[i] = some ? __ldcg(&a.part_ml[at]) : make_float2(-INFINITY, 0.0f);
+        v[i] = some ? __ldcg(reinterpret_cast<const float4*>(a.part_o + at * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+      add(ml, v);
+    }
+  }
+  // the attention's values; a row without a key has zeros
+  __device__ __forceinline__ void finish() {
+    const float norm = sum == 0.0f ? 0.0f : __frcp_rn(sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(y[e], norm);
+  }
+};
 
 // FUSED (tails of one part): the prefix's parts are joined in, and the rows
 // written out.
@@ -320,55 +368,41 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
     const int r = x / (D / 4), d = x % (D / 4) * 4;
     if (row0 + r >= rows) break;
     const size_t unit = (size_t)(token0 + (row0 + r) / a.group) * a.heads + h * a.group + (row0 + r) % a.group;
-    float top = -INFINITY;
+    static_assert(ATT_WARPS == 4, "one step of the sum");
+    Joined sum;
+    float2 ml[4];
+    float4 v[4];
 #pragma unroll
-    for (int w = 0; w < ATT_WARPS; ++w) top = fmaxf(top, sm.ml[w][r].x);
-    if (fused)
-      for (int p = 0; p < a.prefix_parts; ++p) top = fmaxf(top, __ldcg(&a.part_ml[p * stride + unit].x));
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, y[4] = {};
-#pragma unroll
-    for (int w = 0; w < ATT_WARPS; ++w) {
-      const float f = ex2(__fadd_rn(sm.ml[w][r].x, -base));
-      const float4 v = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
-      sum = __fmaf_rn(sm.ml[w][r].y, f, sum);
-      y[0] = __fmaf_rn(v.x, f, y[0]);
-      y[1] = __fmaf_rn(v.y, f, y[1]);
-      y[2] = __fmaf_rn(v.z, f, y[2]);
-      y[3] = __fmaf_rn(v.w, f, y[3]);
+    for (int w = 0; w < 4; ++w) {
+      ml[w] = sm.ml[w][r];
+      v[w] = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
     }
+    sum.add(ml, v);
     if (!fused) {
       const size_t at = index * stride + unit;
-      *reinterpret_cast<float4*>(a.part_o + at * D + d) = make_float4(y[0], y[1], y[2], y[3]);
-      if (d == 0) a.part_ml[at] = make_float2(top, sum);
+      *reinterpret_cast<float4*>(a.part_o + at * D + d) = make_float4(sum.y[0], sum.y[1], sum.y[2], sum.y[3]);
+      if (d == 0) a.part_ml[at] = make_float2(sum.top, sum.sum);
       continue;
     }
-#pragma unroll 4
-    for (int p = 0; p < a.prefix_parts; ++p) {
-      const float2 ml = __ldcg(&a.part_ml[p * stride + unit]);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + (p * stride + unit) * D + d));
-      const float f = ex2(__fadd_rn(ml.x, -base));
-      sum = __fmaf_rn(ml.y, f, sum);
-      y[0] = __fmaf_rn(v.x, f, y[0]);
-      y[1] = __fmaf_rn(v.y, f, y[1]);
-      y[2] = __fmaf_rn(v.z, f, y[2]);
-      y[3] = __fmaf_rn(v.w, f, y[3]);
-    }
-    const float norm = sum == 0.0f ? 0.0f : __frcp_rn(sum);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(y[e], norm);
+    sum.add_parts<D>(a, stride, unit, d, 0, 1, a.prefix_parts);
+    sum.finish();
     const int row = token0 + (row0 + r) / a.group, head = h * a.group + (row0 + r) % a.group;
-    store_out4<BF16>(a.out, a.out_vector, row * a.out.row_stride + head * a.out.head_stride + d, y);
+    store_out4<BF16>(a.out, a.out_vector, row * a.out.row_stride + head * a.out.head_stride + d, sum.y);
   }
 }
 
-// Joins the parts of a row: D / 4 lanes for each (token, head).
+// Joins the parts of a (token, head): D / 4 lanes for each, or for each of
+// `ways` shares of its parts, which are then joined in their order. One lane
+// group over 128 parts took 19 us of a 37 us call (one row of 16384 keys);
+// shares of four parts and more, with four parts' loads in flight, 3 us.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) k_kv_join(AttendDev a) {
-  constexpr int LANES = D / 4;
+__global__ void __launch_bounds__(256) k_kv_join(AttendDev a, int ways) {
+  constexpr int LANES = D / 4, SLOTS = 256 / LANES;
+  __shared__ float4 share_o[SLOTS][LANES];
+  __shared__ float2 share_ml[SLOTS];
   pdl_wait();
-  const int lane = threadIdx.x % LANES;
-  const long long unit = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;
+  const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, way = slot % ways;
+  const long long unit = (long long)blockIdx.x * (SLOTS / ways) + slot / ways;
   const bool some = unit < (long long)a.b.rows * a.heads;
   const int row = some ? (int)(unit / a.heads) : 0, head = some ? (int)(unit % a.heads) : 0;
   // all of a warp's units are of the first one's row or of rows behind it: search for each row that occurs
@@ -380,32 +414,60 @@ __global__ void __launch_bounds__(256) k_kv_join(AttendDev a) {
     left &= ~__ballot_sync(FULL, row == one);
   }
   const Span sp = span_of(a.b, s);
-  if (!some || !sp.ok || row < sp.first || row >= sp.first + sp.n) return;
-  const int parts = a.prefix_parts + a.tail_parts;
+  const bool live = some && sp.ok && row >= sp.first && row < sp.first + sp.n;
+  const int parts = live ? a.prefix_parts + a.tail_parts : 0;
   const size_t stride = (size_t)a.b.rows * a.heads;
-  float top = -INFINITY;
-  for (int p = 0; p < parts; ++p) top = fmaxf(top, a.part_ml[p * stride + unit].x);
-  const float base = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, y[4] = {};
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const float2 ml = a.part_ml[p * stride + unit];
-    const float4 v = *reinterpret_cast<const float4*>(a.part_o + (p * stride + unit) * D + lane * 4);
-    const float f = ex2(__fadd_rn(ml.x, -base));
-    sum = __fmaf_rn(ml.y, f, sum);
-    y[0] = __fmaf_rn(v.x, f, y[0]);
-    y[1] = __fmaf_rn(v.y, f, y[1]);
-    y[2] = __fmaf_rn(v.z, f, y[2]);
-    y[3] = __fmaf_rn(v.w, f, y[3]);
-  }
-  const float norm = sum == 0.0f ? 0.0f : __frcp_rn(sum);
+  Joined sum;
+  sum.add_parts<D>(a, stride, (size_t)unit, lane * 4, way, ways, parts);
+  if (ways > 1) {
+    share_o[slot][lane] = make_float4(sum.y[0], sum.y[1], sum.y[2], sum.y[3]);
+    if (lane == 0) share_ml[slot] = make_float2(sum.top, sum.sum);
+    __syncthreads();
+    if (way) return;
+    for (int w = 1; w < ways; w += 4) {
+      float2 ml[4];
+      float4 v[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(y[e], norm);
-  store_out4<BF16>(a.out, a.out_vector, row * a.out.row_stride + head * a.out.head_stride + lane * 4, y);
+      for (int i = 0; i < 4; ++i) {
+        const bool some = w + i < ways;
+        ml[i] = some ? share_ml[slot + w + i] : make_float2(-INFINITY, 0.0f);
+        v[i] = some ? share_o[slot + w + i][lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+      sum.add(ml, v);
+    }
+  }
+  if (!live) return;
+  sum.finish();
+  store_out4<BF16>(a.out, a.out_vector, row * a.out.row_stride + head * a.out.head_stride + lane * 4, sum.y);
 }
 
 // How a side (the prefix or the tails) is cut: the kernel, its row tiles and
 // its chunks of keys. The same plan sizes the workspace.
+//
+// The plan is the cheapest of all cuts by an estimate in microseconds, whose
+// constants were fitted to both kernels, forced, over 2 to 1024 rows, 256 to
+// 16384 keys and 4 to 1024 lists (4 kv heads):
+//   16 rows:  a CTA's turns (32 keys for each of its four warps) at 1.0 (D = 64)
+//             or 1.4 us, and the codes of all tiles at 4.6 TB/s, as the root of
+//             the sum of squares
+//   128 rows: rounds of one CTA an SM, each 3.5 us and a key tile's time: 1.35
+//             or 1.7 us, for two row tiles 2.85 at either width
+//   a part:   0.1 us, and its bytes twice at 4 TB/s; the join's launch: 4 us
+// Both sides, in us for the call at 4 kv heads, 16 against 128 rows:
+//   1024 shared keys, 64 / 128 rows      D = 64  8.1 / 8.9 against 11.0 / 11.9
+//   16384 shared keys, 64 / 128 rows     D = 128 34 / 54 against 27 / 30
+//   32 sequences of 1024, 16 / 64 rows   D = 64  15 / 26 against 20 / 21
+//   32 sequences of 8192, 16 / 64 rows   D = 128 94 / 244 against 144 / 149
+// and one against two row tiles of 128:
+//   16 sequences of 4096, 256 rows       57 against 59 (D = 64), 82 against 71 (D = 128)
+//   16384 shared keys, 256 / 1024 rows   D = 128 40 / 104 against 44 / 97
+constexpr double PLAN_PART = 0.1, PLAN_JOIN = 4.0;
+
+// Up to this many parts of the prefix are joined by the tails' own CTAs, more
+// by the join's launch. 512 and 2048 shared keys for one row (4 and 16 parts):
+// 5.1 and 6.5 us against 7.1 and 7.3; 32768 keys for 5 rows: 20.5 against 15.7.
+constexpr int FUSED_PARTS = 16;
+
 struct SidePlan {
   bool wide = false, pair = false;
   int tiles = 0;   // row tiles (prefix: of the batch, tails: of a sequence)
@@ -413,41 +475,42 @@ struct SidePlan {
   int chunk = 32, parts = 0;
 };
 
-constexpr int WIDE_FROM = 33;  // rows that meet the same keys
-
 // rows: query rows (token, head of the group) that meet the same `keys`;
 // `lists`: how many such sets there are (kv heads, times sequences).
-static SidePlan side_plan(long long rows, int keys, long long lists, size_t part_bytes) {
-  SidePlan p;
-  p.wide = rows >= WIDE_FROM;
-  p.pair = rows > 128;
-  const int cover = p.wide ? (p.pair ? 256 : 128) : 16, unit = p.wide ? 128 : 32;
-  p.tiles = (int)((rows + cover - 1) / cover);
-  if (keys == 0 || lists == 0 || p.tiles == 0) return p;
-  const int units = (keys + unit - 1) / unit;
-  int chunks = 1;
-  if (p.wide) {
-    // one CTA an SM: the fewest rounds of key tiles, with the time of a tile
-    // (about 1 us) against that of writing and joining one more part
-    double best = 0;
-    for (int n = 1; n <= units && n <= 64; ++n) {
-      const long long rounds = (lists * p.tiles * n + 147) / 148;
-      const double cost = (double)rounds * ((units + n - 1) / n + 2) + (double)n * (p.pair ? 1 : 2) * part_bytes * 2 / 4e6;
-      if (n == 1 || cost < best) {
-        best = cost;
-        chunks = n;
-      }
-    }
-  } else {
-    // small CTAs, about four an SM, of at least 128 keys
-    const long long want = (4 * 148 + lists * p.tiles - 1) / (lists * p.tiles);
-    chunks = (int)(want > (units + 3) / 4 ? (units + 3) / 4 : want);
+static SidePlan side_plan(long long rows, int keys, long long lists, int dim, bool tail, size_t part_bytes) {
+  SidePlan best;
+  best.tiles = (int)((rows + 15) / 16);
+  if (keys == 0 || lists == 0 || rows == 0) return best;
+  double best_us = 0;
+  // a part is written and read again, and joined in its turn
+  const double part_us = PLAN_PART + part_bytes * 2 / 4e6;
+  auto take = [&](double us, bool wide, bool pair, int tiles, int units, int chunks) {
+    if (best.chunks && us >= best_us) return;
+    best_us = us;
+    const int unit = wide ? 128 : 32, each = (units + chunks - 1) / chunks;
+    best.wide = wide;
+    best.pair = pair;
+    best.tiles = tiles;
+    best.chunk = each * unit;
+    best.chunks = (units + each - 1) / each;
+    best.parts = best.chunks * (wide && !pair ? 2 : 1);
+  };
+  const int groups = (keys + 31) / 32, units = (keys + 127) / 128;
+  const long long narrow = (rows + 15) / 16;
+  const double bytes_us = (double)lists * narrow * keys * (2 * dim) / 4.6e6;
+  for (int n = 1; n <= groups && n <= 64 && (n == 1 || n * part_us < best_us); ++n) {
+    const double turns = ((groups + n - 1) / n + ATT_WARPS - 1) / ATT_WARPS * (dim == 64 ? 1.0 : 1.4);
+    take(std::sqrt(turns * turns + bytes_us * bytes_us) + n * part_us + (tail && n == 1 ? 0.0 : PLAN_JOIN), false, false, (int)narrow, groups, n);
   }
-  const int each = (units + chunks - 1) / chunks;
-  p.chunk = each * unit;
-  p.chunks = (units + each - 1) / each;
-  p.parts = p.chunks * (p.wide && !p.pair ? 2 : 1);
-  return p;
+  for (int pair = 0; pair < (rows > 128 ? 2 : 1); ++pair) {
+    const long long tiles = (rows + (pair ? 255 : 127)) / (pair ? 256 : 128);
+    const double tile_us = pair ? 2.85 : dim == 64 ? 1.35 : 1.7;
+    for (int n = 1; n <= units && n <= 64 && n * part_us < best_us; ++n) {
+      const long long rounds = (lists * tiles * n + 147) / 148;
+      take((double)rounds * ((units + n - 1) / n * tile_us + 3.5) + n * (pair ? 1 : 2) * part_us + PLAN_JOIN, true, pair, (int)tiles, units, n);
+    }
+  }
+  return best;
 }
 
 struct AttendPlan {
@@ -458,8 +521,8 @@ static AttendPlan attend_plan(const KvCacheDev& c, const KvBatchDev& b, int pref
   const long long group = heads / c.kv_heads;
   const size_t part_bytes = (size_t)b.rows * heads * c.dim * sizeof(float);
   AttendPlan p;
-  p.prefix = side_plan(b.rows * group, prefix, c.kv_heads, part_bytes);
-  p.tail = side_plan(b.max_rows * group, b.max_length, (long long)b.sequences * c.kv_heads, part_bytes);
+  p.prefix = side_plan(b.rows * group, prefix, c.kv_heads, c.dim, false, part_bytes);
+  p.tail = side_plan(b.max_rows * group, b.max_length, (long long)b.sequences * c.kv_heads, c.dim, true, part_bytes);
   return p;
 }
 
@@ -504,15 +567,21 @@ static cudaError_t attend_launch(const AttendDev& d, const AttendPlan& p, cudaSt
   bool fused = false;
   if (e == cudaSuccess && p.tail.chunks) {
     const unsigned tiles = (unsigned)d.b.sequences * p.tail.tiles;
-    fused = !p.tail.wide && p.tail.parts == 1;
+    fused = !p.tail.wide && p.tail.parts == 1 && p.prefix.parts <= FUSED_PARTS;
     if (p.tail.wide)
       e = attend_wide(d, false, (int)tiles, p.tail.chunks, before, st);
     else
       e = launch(k_kv_attend<D, BF16, E4M3, false>, dim3(tiles, d.c.kv_heads, p.tail.chunks), ATT_WARPS * 32, SMEM, before, st, d, fused);
     before = true;
   }
-  if (e == cudaSuccess && !fused)
-    e = launch(k_kv_join<D, BF16>, dim3((unsigned)(((long long)d.b.rows * d.heads * (D / 4) + 255) / 256)), 256, 0, before, st, d);
+  if (e == cudaSuccess && !fused) {
+    constexpr int SLOTS = 256 / (D / 4);
+    const long long units = (long long)d.b.rows * d.heads;
+    int ways = 1;
+    while (ways < SLOTS && (d.prefix_parts + d.tail_parts) >= 8 * ways && units * ways < 148 * 4 * SLOTS) ways *= 2;
+    const int each = SLOTS / ways;  // units a block
+    e = launch(k_kv_join<D, BF16>, dim3((unsigned)((units + each - 1) / each)), 256, 0, before, st, d, ways);
+  }
   return e;
 }
 

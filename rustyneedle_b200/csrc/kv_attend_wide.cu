@@ -16,18 +16,23 @@
 // The softmax reads TMEM in 16-lane pieces of 256 bits a row, so a thread has
 // 4 rows x 32 keys of the tile (rows lane / 4 + 8 k, keys 8 n + 2 (lane % 4)
 // and the next), not 1 x 128: a key's numbers (scale, the value scale's
-// logarithm and reciprocal) then serve 4 rows of a thread. Shared memory's 128
-// bytes a cycle are what is short here: for a tile pair at D = 128 the matrix
-// operands take 1536 cycles, the loaders' stores 512 and the keys' numbers 768;
-// with a row a thread they took 3072.
+// logarithm and reciprocal) then serve 4 rows of a thread, a quarter of the
+// shared-memory reads.
 //
 // O is rescaled in TMEM only when a row's maximum has grown by more than
 // SLACK: until then the weights just get larger, up to 2^(HEADROOM + SLACK).
 //
 // Per 128 keys and slot: 4 · 128 · 128 · D flops on the tensor cores (512
-// cycles at D = 64, 1024 at D = 128), 16384 exponentials (1024 cycles of the
-// special-function units), so at D = 64 the exponentials bound the kernel and
-// at D = 128 both are even.
+// cycles at D = 64, 1024 at D = 128) and 16384 exponentials (1024 cycles of the
+// special-function units). Measured at 40000 shared keys, 512 rows of 8 kv
+// heads, D = 128: 139 us, about 6700 cycles for a key tile of two slots, whose
+// matrix instructions take 2048. No single unit is what it waits for: copies
+// without the exponentials, the maximum, the weights, the widening, the global
+// loads or one of the two products were 0 to 19% faster each, and one without
+// all of them still took 65 us, the chain of hand-offs from score to weights to
+// product. More slots would fill it, but two have all of TMEM at D = 128;
+// key tiles of 64 with two score buffers a slot were slower (161 us), as were
+// an issuing warp for each slot (145) and 16 softmax warps (147).
 #include "kv_attend.cuh"
 
 namespace nbk {
@@ -42,10 +47,9 @@ __device__ __forceinline__ uint64_t core_desc(uint32_t addr, uint32_t sbo) {
   return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)((sbo >> 4) & 0x3fff) << 32) | (1ull << 46);
 }
 
-// The issuing warp runs as a whole, its operands the same in every lane (so
-// that they live in uniform registers: through one lane's vector registers an
-// event's instructions took 1850 cycles, three times their execution), and one
-// elected lane issues.
+// The issuing warp runs as a whole, its operands the same in every lane, so
+// that they can live in uniform registers, and one elected lane issues: 170 us
+// for a call that took 174 with one lane of a diverged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t leader;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(leader));
@@ -66,9 +70,8 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// One arrival for a warp: 32 lanes' arrivals on one barrier are served one
-// after another, and with a few hundred of them a tile they were what took
-// the time.
+// One arrival for a warp: a call of long questions took 133 us, with an
+// arrival from every lane (several hundred a tile) 141.
 __device__ __forceinline__ void warp_arrive(uint32_t bar) {
   __syncwarp();
   if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");

@@ -530,8 +530,11 @@ template <typename T, int D, bool E4M3>
 static cudaError_t rows_launch(bool append, const KvCacheDev& c, const KvBatchDev& b, const RowsDev& keys, const RowsDev& values, cudaStream_t st) {
   const bool vector = aligned_rows(keys, sizeof(T), D / 32) && aligned_rows(values, sizeof(T), D / 32);
   // Blocks of rows where most of them can lie in one sequence and page, and
-  // there are enough of them to fill the SMs.
-  if (b.max_rows >= 2 * BLOCK_ROWS && (long long)b.rows * c.kv_heads >= 148 * 16 * BLOCK_ROWS / 2) {
+  // there are enough of them to fill the SMs. A row a warp against blocks, in us:
+  //   one sequence, 4 heads of 64:   4096 rows 8.8 : 10.5 append, 5.5 : 5.4 read; 8192 13.5 : 11.6, 8.7 : 6.0
+  //   one sequence, 8 heads of 128:  2048 rows 12.2 : 14.3, 6.8 : 7.3; 4096 21.3 : 15.8, 11.1 : 8.2
+  //   32768 rows of 8 heads of 128, sequences of 8: 148 : 148, 95 : 71; of 16: 148 : 124, 92 : 50
+  if (b.max_rows >= BLOCK_ROWS && (long long)b.rows * c.kv_heads >= 148 * 16 * BLOCK_ROWS / 2) {
     // a lane's D / 16 elements in accesses of at most 16 bytes
     const bool vector16 = aligned_rows(keys, sizeof(T), D / 16) && aligned_rows(values, sizeof(T), D / 16);
     const unsigned blocks = (unsigned)((b.rows + BLOCK_ROWS * ROW_WARPS - 1) / (BLOCK_ROWS * ROW_WARPS)) * c.kv_heads;
@@ -541,7 +544,9 @@ static cudaError_t rows_launch(bool append, const KvCacheDev& c, const KvBatchDe
       k_kv_read_block<T, D, E4M3><<<blocks, ROW_WARPS * 32, 0, st>>>(c, b, keys, values, vector16);
     return cudaGetLastError();
   }
-  // all units of a row for a warp, unless that leaves SMs short of warps (16 each)
+  // all units of a row for a warp, unless that leaves SMs short of warps (16
+  // each): one row of 8 heads of 128 took 9.8 us with all of them and 3.9 with
+  // four a warp, 4096 rows of 64 heads 192 and 203.
   const int units = c.kv_heads * 2;
   int each = (units + 3) / 4 * 4;
   while (each > 4 && (long long)b.rows * ((units + each - 1) / each) < 148 * 16) each = (each / 2 + 3) / 4 * 4;

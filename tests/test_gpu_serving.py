@@ -52,7 +52,7 @@ def paged(rng, lengths, before=0, spare=3):
     return order[:before].copy(), table, total
 
 
-def make_batch(nb, torch, rows, lengths, table, **more):
+def make_batch(nb, torch, rows, lengths, table, /, **more):
     more = {"rows": int(sum(rows)), "max_rows": int(max(rows, default=0)), "max_length": int(max(lengths, default=0)), **more}
     return nb.KvBatch(int32(torch, starts(rows)), int32(torch, lengths), int32(torch, table), **more)
 
@@ -233,8 +233,9 @@ def test_bad_pages_and_sequences_are_left_out_and_reported(nb, torch):
 # -------------------------------------------------------------------------------------------------------------- attend
 
 
-def check_attend(nb, torch, cache, query, keys, values, rows, lengths, table, prefix=0, prefix_pages=None, scale=None, out=None):
-    """Attends and compares. keys and values hold the prefix's rows, then all positions of each sequence.
+def check_attend(nb, torch, cache, query, keys, values, rows, lengths, table, prefix=0, prefix_pages=None, scale=None, out=None, bounds=None):
+    """Attends and compares. keys and values hold the prefix's rows, then all positions of each sequence. `bounds` are the
+    batch's, above its own.
 
     The bound for one element, to first order:
       half a step of the output's type, relative: eps / 2
@@ -247,7 +248,7 @@ def check_attend(nb, torch, cache, query, keys, values, rows, lengths, table, pr
     scale_ = 1 / math.sqrt(query.shape[2]) if scale is None else scale
     n = sum(rows)
     result = torch.full_like(query, 3.0) if out is None else out
-    batch = make_batch(nb, torch, rows, lengths, table)
+    batch = make_batch(nb, torch, rows, lengths, table, **(bounds or {}))
     cache.attend(batch, query, result, prefix_pages, prefix, scale)
     cache.check()
     kc, ks = ref.quantise(numbers(keys), cache.format)
@@ -265,13 +266,13 @@ def check_attend(nb, torch, cache, query, keys, values, rows, lengths, table, pr
     return result
 
 
-def attend_case(nb, torch, seed, rows, lengths, prefix, heads, kv, dim, kind, dtype, strided=False, scale=None, change=None):
+def attend_case(nb, torch, seed, rows, lengths, prefix, heads, kv, dim, kind, dtype, strided=False, scale=None, change=None, bounds=None):
     rng = np.random.default_rng(seed)
     t = dtype_of(torch, dtype)
     prefix_pages, table, pages = paged(rng, lengths, -(-prefix // PAGE))
     keys = random_rows(rng, torch, prefix + sum(lengths), kv, dim, t)
     values = random_rows(rng, torch, prefix + sum(lengths), kv, dim, t)
-    query = random_rows(rng, torch, sum(rows) + 1, heads, dim, t, strided)
+    query = random_rows(rng, torch, (bounds or {}).get("rows", sum(rows) + 1), heads, dim, t, strided)
     if change:
         change(query, keys, values)
     cache = nb.KvCache(kv, dim, pages, format=kind, device=0)
@@ -282,8 +283,8 @@ def attend_case(nb, torch, seed, rows, lengths, prefix, heads, kv, dim, kind, dt
         cache.append(make_batch(nb, torch, lengths, lengths, table), keys[prefix:], values[prefix:])
     out = torch.full_like(query, 3.0)
     if strided:
-        out = torch.full((heads, sum(rows) + 1, dim + 2), 3.0, dtype=t, device="cuda:0")[:, :, :dim].transpose(0, 1)
-    return check_attend(nb, torch, cache, query, keys, values, rows, lengths, table, prefix, shared, scale, out)
+        out = torch.full((heads, query.shape[0], dim + 2), 3.0, dtype=t, device="cuda:0")[:, :, :dim].transpose(0, 1)
+    return check_attend(nb, torch, cache, query, keys, values, rows, lengths, table, prefix, shared, scale, out, bounds)
 
 
 ATTEND_CASES = [  # rows, lengths, prefix, heads, kv heads
@@ -301,6 +302,27 @@ ATTEND_CASES = [  # rows, lengths, prefix, heads, kv heads
 def test_attend(nb, torch, kind, dtype, dim, case):
     rows, lengths, prefix, heads, kv = ATTEND_CASES[case]
     attend_case(nb, torch, 200 + case, rows, lengths, prefix, heads, kv, dim, kind, dtype, strided=case % 4 == 1)
+
+
+# The kernel, its tiles and its split follow the batch's bounds: with these the tiles of 128 rows are taken for sequences
+# and prefixes of any length, one tile or two to a block.
+WIDE_BOUNDS = [{"rows": 8192, "max_rows": 2048, "max_length": 1 << 14}, {"rows": 4000, "max_rows": 150, "max_length": 1 << 17}]
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("case", range(len(ATTEND_CASES)))
+def test_attend_with_wide_bounds(nb, torch, kind, dtype, dim, case):
+    rows, lengths, prefix, heads, kv = ATTEND_CASES[case]
+    attend_case(nb, torch, 250 + case, rows, lengths, prefix, heads, kv, dim, kind, dtype, strided=case % 4 == 2, bounds=WIDE_BOUNDS[case % 2])
+
+
+@pytest.mark.parametrize("prefix", [1, 127, 128, 129, 255, 256, 257, 383, 640, 1025])
+@pytest.mark.parametrize("tail", [1, 127, 128, 129, 257, 400])
+def test_attend_at_the_edges_of_wide_tiles(nb, torch, prefix, tail):
+    n, odd = prefix + tail, prefix % 2
+    attend_case(nb, torch, n, [min(tail, 130), 1, min(tail, 64)], [tail, 1, tail], prefix, 4, 2, 64 if odd else 128, "int8" if tail % 2 else "e4m3", "fp16", bounds=WIDE_BOUNDS[n % 2])
 
 
 @pytest.mark.parametrize("prefix", [127, 128, 129, 255, 256, 257, 383, 1025])
@@ -367,6 +389,77 @@ def test_attend_does_not_look_behind_the_end(nb, torch, rows, kind):
 def test_attend_long_tails_and_a_long_prefix(nb, torch):
     attend_case(nb, torch, 45, [1, 2], [20000, 5000], 0, 4, 1, 64, "int8", "bf16")
     attend_case(nb, torch, 46, [1, 1], [1, 70], 30000, 4, 1, 128, "e4m3", "fp16")
+
+
+def test_attend_many_keys_and_many_rows(nb, torch):
+    """The largest tiles over more than one round of key tiles; parts joined in several shares."""
+    attend_case(nb, torch, 52, [600, 1], [5000, 77], 0, 4, 2, 128, "int8", "bf16")
+    attend_case(nb, torch, 53, [1] * 300, [3] * 300, 5000, 8, 2, 64, "e4m3", "fp16")
+    attend_case(nb, torch, 54, [1], [70], 60000, 4, 1, 64, "int8", "bf16")
+    attend_case(nb, torch, 55, [2] * 5, [9000 + 64 * i for i in range(5)], 0, 2, 2, 64, "int8", "fp16")
+
+
+def test_attend_a_row_that_could_not_be_held_with_wide_bounds(nb, torch):
+    def change(query, keys, values):
+        keys[100 + 20, 0, 3] = float("nan")
+        values[100 + 25, 1, 3] = float("inf")
+
+    for bounds in WIDE_BOUNDS:
+        out = numbers(attend_case(nb, torch, 56, [30, 30], [30, 30], 100, 4, 2, 128, "int8", "bf16", change=change, bounds=bounds)[:60])
+        assert np.isnan(out[20:30, :2]).all() and np.isfinite(out[:20, :2]).all()
+        assert np.isnan(out[25:30, 2:]).all() and np.isfinite(out[:25, 2:]).all() and np.isfinite(out[30:]).all()
+
+
+def test_attend_with_wide_bounds_does_not_look_behind_the_end(nb, torch):
+    rng = np.random.default_rng(57)
+    kv, dim, prefix, rows = 2, 128, 70, 40
+    length = rows + 9
+    prefix_pages, table, pages = paged(rng, [length + 150], -(-(prefix + 100) // PAGE))
+    cache = nb.KvCache(kv, dim, pages, format="e4m3", device=0)
+    poison = torch.full((length + 400, kv, dim), float("nan"), dtype=torch.bfloat16, device="cuda:0")
+    cache.append(make_batch(nb, torch, [prefix + 50], [prefix + 50], prefix_pages[None]), poison, poison)
+    cache.append(make_batch(nb, torch, [length + 150], [length + 150], table), poison, poison)
+    keys, values = (random_rows(rng, torch, prefix + length, kv, dim, torch.bfloat16) for _ in range(2))
+    cache.append(make_batch(nb, torch, [prefix], [prefix], prefix_pages[None]), keys[:prefix], values[:prefix])
+    cache.append(make_batch(nb, torch, [length], [length], table), keys[prefix:], values[prefix:])
+    for bounds in WIDE_BOUNDS:
+        query = random_rows(rng, torch, bounds["rows"], 4, dim, torch.bfloat16)
+        check_attend(nb, torch, cache, query, keys, values, [rows], [length], table, prefix, int32(torch, prefix_pages), bounds=bounds)
+
+
+def test_attend_with_wide_bounds_leaves_out_bad_pages_and_sequences(nb, torch):
+    """A page outside the pool counts as no keys, in the prefix and in a tail; a sequence out of its bounds gets nothing."""
+    rng = np.random.default_rng(58)
+    kv, dim = 2, 128
+    cache = nb.KvCache(kv, dim, 8, device=0)
+    keys, values = (random_rows(rng, torch, 128, kv, dim, torch.bfloat16) for _ in range(2))
+    cache.append(make_batch(nb, torch, [128], [128], np.array([[0, 1]])), keys, values)
+    for bounds in WIDE_BOUNDS:
+        query = random_rows(rng, torch, bounds["rows"], 4, dim, torch.bfloat16)
+        whole, part = (torch.full_like(query, 5.0) for _ in range(2))
+        for result, table, prefix_pages in ((whole, [[0]], [1]), (part, [[0, 1000]], [1, -1])):
+            batch = make_batch(nb, torch, [40], [64], np.array(table), **bounds)
+            cache.attend(batch, query, result, int32(torch, prefix_pages), 64)
+        cache.check()
+        assert torch.equal(whole, part)
+        batch = make_batch(nb, torch, [40], [100], np.array([[0, 1000]]), **bounds)  # rows 60 .. 99 of the 100 positions
+        cache.attend(batch, query, part, int32(torch, [1, -1]), 128)
+        with pytest.raises(nb.NeedleError):
+            cache.check()
+        cache.attend(make_batch(nb, torch, [40], [64], np.array([[0]]), **bounds), query, whole, int32(torch, [1]), 64)
+        cache.check()
+        # rows 60 .. 99 see all of the 64 positions whose page is there, and so does row 63 of the other batch. The prefixes'
+        # lengths split the keys differently, so both are off from the same value by their own roundings: half a step of
+        # bf16 each (2^-8 of a value no larger than the largest in the cache), and the f16 weights' 2^-11 each
+        assert float((part[39] - whole[39]).abs().max()) <= (2 * 2.0**-8 + 2 * 2.0**-10) * float(values.abs().max())
+        assert bool((part[40:] == 5.0).all())
+        mixed = make_batch(nb, torch, [3, 40, 2], [10, 3, 20], np.array([[0], [1], [0]]), **bounds)
+        part.fill_(5.0)
+        cache.attend(mixed, query, part, int32(torch, [1]), 64)
+        with pytest.raises(nb.NeedleError) as e:
+            cache.check()
+        assert "sequence" in e.value.message
+        assert bool((part[3:43] == 5.0).all()) and bool((part[45:] == 5.0).all()) and not bool((part[:3] == 5.0).any()) and not bool((part[43:45] == 5.0).any())
 
 
 def test_attend_is_the_same_every_time(nb, torch):
@@ -617,6 +710,41 @@ def test_verify_strange_logits(nb, torch):
     check_verify(nb, torch, x)
     x["temperature"] = 1e30
     check_verify(nb, torch, x)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("temperature", [0.0, 0.7, 1.0])
+def test_verify_logits_masked_with_the_lowest_value(nb, torch, dtype, temperature):
+    """Masks written into the logits: the type's lowest value, -inf, both, in all places but one and in all."""
+    rng = np.random.default_rng(65)
+    x = verify_inputs(rng, torch, 9, 2, 517, dtype, temperature=temperature)
+    l = x["logits"]
+    low = torch.finfo(l.dtype).min
+    drop = torch.tensor(rng.random(l.shape) < 0.7, device="cuda:0")
+    drop[2], drop[3], drop[6] = True, True, True
+    drop[3, :, 400] = False
+    l[:4] = torch.where(drop[:4], torch.full_like(l[:4], low), l[:4])
+    l[4:7] = torch.where(drop[4:7], torch.full_like(l[4:7], float("-inf")), l[4:7])
+    l[7, :, ::2], l[7, :, 1::2] = low, float("-inf")
+    l[8], l[8, 0, 3] = low, torch.finfo(l.dtype).max
+    check_verify(nb, torch, x)
+
+
+@pytest.mark.parametrize("drafts", [63, 64, 65, 130])
+def test_verify_many_drafts(nb, torch, drafts):
+    """More drafts than a block holds at once, with runs that are accepted to the end and runs that are not."""
+    rng = np.random.default_rng(66)
+    for given, temperature in ((True, 1.0), (False, 1.0), (False, 0.0)):
+        x = verify_inputs(rng, torch, 5, drafts, 130, "fp32", given=given, temperature=temperature, noise=0.05)
+        if given:
+            x["accept"] *= 0.9
+        else:
+            x["accept"][:3] = 0.0
+        if temperature == 0:
+            x["tokens"][:3] = x["logits"][:3, :drafts].argmax(-1).cpu().numpy()
+        counts = [drafts, drafts - 1, min(drafts, 64), drafts, 0]
+        check_verify(nb, torch, x)
+        check_verify(nb, torch, x, np.array(counts, dtype=np.int32))
 
 
 def test_verify_uniforms_at_their_ends(nb, torch):
