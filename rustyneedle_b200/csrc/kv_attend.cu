@@ -45,7 +45,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // keys 4·(n / 2) + 2·j + n % 2, which leaves lane c the scores of the keys 4c
 // .. 4c + 3: the order in which the second product wants its left operand, and
 // in which the pool keeps the values (value_byte).
-constexpr int ATT_WARPS = 4, ATT_STAGES = 3;
+constexpr int ATT_WARPS = 4, ATT_STAGES = 2;
 
 template <int D>
 struct AttStage {
@@ -239,6 +239,8 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
       }
   }
 
+  // the tile's upper 8 rows hold something; without them half the softmax is left out
+  const bool upper = rows - row0 > 8;
   float o[NT][4] = {};
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   bool fine = true;
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
             inv[blk][e] = key < k1 ? rcp_fast(vscale[e]) : 0.0f;
             // a key that a row does not see gets -inf by selection, whatever lies there
             t[blk][j][e2] = key < limit[0] ? __fmaf_rn(s[e2], mul, add) : -INFINITY;
-            t[blk][j][2 + e2] = key < limit[1] ? __fmaf_rn(s[2 + e2], mul, add) : -INFINITY;
+            if (upper) t[blk][j][2 + e2] = key < limit[1] ? __fmaf_rn(s[2 + e2], mul, add) : -INFINITY;
           }
         }
       }
@@ -285,6 +287,7 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
       float next[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
+        if (half && !upper) break;
         float top = -INFINITY;
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
@@ -299,6 +302,7 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
       if (__any_sync(FULL, grown)) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
+          if (half && !upper) break;
           const float keep = ex2(__fadd_rn(m[half], -base[half]));  // 0 while nothing was seen
           m[half] = next[half];
           l[half] = __fmul_rn(l[half], keep);
@@ -310,7 +314,8 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
         }
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int half = 0; half < 2; ++half) {
+        if (half && !upper) break;
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
@@ -322,10 +327,11 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
               x = ex2(__fadd_rn(x, -base[half]));
               l[half] = seen ? __fmaf_rn(x, inv[blk][2 * j + e2], l[half]) : l[half];
             }
+      }
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
-        const uint32_t pf[4] = {pack_f16(t[blk][0][0], t[blk][0][1]), pack_f16(t[blk][0][2], t[blk][0][3]), pack_f16(t[blk][1][0], t[blk][1][1]),
-                                pack_f16(t[blk][1][2], t[blk][1][3])};
+        const uint32_t pf[4] = {pack_f16(t[blk][0][0], t[blk][0][1]), upper ? pack_f16(t[blk][0][2], t[blk][0][3]) : 0u, pack_f16(t[blk][1][0], t[blk][1][1]),
+                                upper ? pack_f16(t[blk][1][2], t[blk][1][3]) : 0u};
 #pragma unroll
         for (int tq = 0; tq < D / 32; ++tq) {
           const uint4 w = *reinterpret_cast<const uint4*>(stage.v + blk * 16 * D + tq * 512 + lane * 16);
