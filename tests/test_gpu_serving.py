@@ -730,6 +730,32 @@ def test_verify_logits_masked_with_the_lowest_value(nb, torch, dtype, temperatur
     check_verify(nb, torch, x)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_verify_greedy_takes_the_lowest_of_equal_maxima(nb, torch, dtype):
+    """Equal maxima, infinities behind NaNs, rows of NaN or -inf alone, in rows long enough for every thread's steps."""
+    rng = np.random.default_rng(67)
+    for vocab in (40000, 40011):
+        x = verify_inputs(rng, torch, 8, 3, vocab, dtype, given=False, temperature=0.0)
+        l = x["logits"]
+        top = torch.finfo(l.dtype).max
+        l[0, :, 777] = l[0, :, 30001] = 60.0
+        l[1, :, 5000] = l[1, :, 20000] = float("inf")
+        l[1, :, 4990:5000] = float("nan")
+        l[2, :, 9] = float("nan")
+        l[2, :, 100] = l[2, :, 39999] = top
+        l[2, :, 35000] = float("inf")
+        l[3] = float("nan")
+        l[3, 0, 39990] = -5.0
+        l[4] = float("-inf")
+        l[4, 0, 12345] = torch.finfo(l.dtype).min
+        l[5] = 0.0
+        l[6] = -0.0
+        l[6, :, 3333] = 0.0
+        l[7, :, 1:] = torch.sort(l[7, :, 1:], dim=-1).values  # the maximum grows with every step
+        x["tokens"][:] = l[:, :3].float().nan_to_num(nan=float("-inf"), posinf=float("inf")).argmax(-1).cpu().numpy()
+        check_verify(nb, torch, x)
+
+
 @pytest.mark.parametrize("drafts", [63, 64, 65, 130])
 def test_verify_many_drafts(nb, torch, drafts):
     """More drafts than a block holds at once, with runs that are accepted to the end and runs that are not."""
