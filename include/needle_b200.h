@@ -372,7 +372,8 @@ nb_status nb_kv_cache_attend_workspace(const nb_kv_cache* cache, const nb_kv_bat
  * with k_j and v_j the values that the cache holds. A row without any visible
  * position (its pages outside the pool) gets zeros. query and out are
  * [rows][heads][head_dim], both NB_F16 or both NB_BF16; heads is a multiple of
- * kv_heads, at most 64 for each. The prefix is read once for the whole batch.
+ * kv_heads, at most 64 for each. The prefix is gone through for the rows of the
+ * whole batch together, not for each sequence.
  * The tail's new rows have to be in the cache (nb_kv_cache_append, earlier on
  * the same stream). Sums, maxima and products are accumulated in f32; the
  * probabilities enter their product with the codes as f16. `workspace` is

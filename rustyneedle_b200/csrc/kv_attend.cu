@@ -9,6 +9,7 @@
 // softmax's own sum. m is the running maximum of t less HEADROOM, so w_j ≤
 // 2^HEADROOM; the product with the codes takes w as f16 (2^-12 relative down
 // to 2^-14, absolute 2^-25 below), the sums take it as f32.
+#include <algorithm>
 #include <cmath>
 
 #include "kv_attend.cuh"
@@ -528,7 +529,8 @@ static AttendPlan attend_plan(const KvCacheDev& c, const KvBatchDev& b, int pref
   const size_t part_bytes = (size_t)b.rows * heads * c.dim * sizeof(float);
   AttendPlan p;
   p.prefix = side_plan(b.rows * group, prefix, c.kv_heads, c.dim, false, part_bytes);
-  p.tail = side_plan(b.max_rows * group, b.max_length, (long long)b.sequences * c.kv_heads, c.dim, true, part_bytes);
+  // also for bounds of no rows or no positions: the tails' kernel reports the sequences that break them
+  p.tail = side_plan(std::max(b.max_rows, 1) * group, std::max(b.max_length, 1), (long long)b.sequences * c.kv_heads, c.dim, true, part_bytes);
   return p;
 }
 

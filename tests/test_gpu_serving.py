@@ -462,6 +462,38 @@ def test_attend_with_wide_bounds_leaves_out_bad_pages_and_sequences(nb, torch):
         assert bool((part[3:43] == 5.0).all()) and bool((part[45:] == 5.0).all()) and not bool((part[:3] == 5.0).any()) and not bool((part[43:45] == 5.0).any())
 
 
+@pytest.mark.parametrize("bounds", [{"max_length": 0}, {"max_rows": 0}, {"max_rows": 0, "max_length": 0}, {"rows": 1}])
+def test_bounds_below_what_the_sequences_have(nb, torch, bounds):
+    """Nothing is written, and it is reported, with and without a prefix."""
+    cache = nb.KvCache(2, 64, 4, device=0)
+    x, y = (torch.ones(2, h, 64, dtype=torch.bfloat16, device="cuda:0") for h in (2, 4))
+    for prefix in (0, 70):
+        out = torch.full_like(y, 5.0)
+        cache.attend(make_batch(nb, torch, [2], [2], np.array([[0]]), **bounds), y, out, int32(torch, [1, 2]), prefix)
+        with pytest.raises(nb.NeedleError) as e:
+            cache.check()
+        assert "sequence" in e.value.message and bool((out == 5.0).all())
+    cache.append(make_batch(nb, torch, [2], [2], np.array([[0]]), **bounds), x, x)
+    with pytest.raises(nb.NeedleError):
+        cache.check()
+
+
+def test_attend_in_place(nb, torch):
+    """The output may be the query itself: every row and head is read before it is written."""
+    rng = np.random.default_rng(59)
+    cache = nb.KvCache(2, 64, 80, device=0)
+    keys, values = (random_rows(rng, torch, 5000, 2, 64, torch.bfloat16) for _ in range(2))
+    cache.append(make_batch(nb, torch, [5000], [5000], np.arange(79)[None]), keys, values)
+    for n, length, prefix in ((1, 5, 100), (40, 300, 1000), (1, 5000, 0), (600, 5000, 2000)):
+        query = random_rows(rng, torch, n, 8, 64, torch.bfloat16)
+        batch = make_batch(nb, torch, [n], [length], np.arange(79)[None])
+        want = torch.empty_like(query)
+        cache.attend(batch, query, want, int32(torch, range(79)), prefix)
+        cache.attend(batch, query, query, int32(torch, range(79)), prefix)
+        assert torch.equal(query, want)
+    cache.check()
+
+
 def test_attend_is_the_same_every_time(nb, torch):
     a, b = (attend_case(nb, torch, 47, [3] * 50, [100 + i for i in range(50)], 900, 8, 2, 128, "int8", "bf16") for _ in range(2))
     assert torch.equal(a, b)
