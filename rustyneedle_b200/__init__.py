@@ -4,6 +4,10 @@ The compute path is the in-tree native library (``_native/libneedle_b200.so``,
 sm_100a kernels behind the C ABI of ``include/needle_b200.h``). There is no CPU
 fallback: when the library is missing, importing the native layer raises.
 
+KvCache, KvBatch and verify_drafts (drafted decoding over a shared prompt, for
+callers with a model of their own) have no seam in the reference; they take
+torch tensors.
+
 Reference seams mirrored here (paths inside the rustyneedle workspace):
   Model.open / Model.with_depth      crates/model/src/model.rs:52-66
   Session.feed / push / logits / len crates/model/src/session.rs:44-177
