@@ -114,7 +114,7 @@ constexpr int ROW_WARPS = 8, ROW_AHEAD = 4;
 // far (two steps of the search, the span, the page), about 3 us, against 256
 // bytes a unit: with a warp for each unit 24000 rows of 8 heads of 128 took
 // 135 us to append and 111 to read, with a warp for a row, 4 units at a time,
-// 97 and 70 (62 and 35 by the blocks of 16 rows below: 2.4 and 4.3 TB/s).
+// 97 and 70 (59 and 35 by the blocks of 16 rows below: 2.5 and 4.3 TB/s).
 struct RowPlace {
   size_t block;  // of head 0 in the pool
   int at;        // position within the page
@@ -338,8 +338,10 @@ __device__ __forceinline__ uint32_t peak_bits(const float (&x)[N]) {
 // A half warp a row: lanes 0 - 15 rows 0 - 7, lanes 16 - 31 rows 8 - 15, D / 16
 // dimensions a lane. grid ceil(rows / 16 / 8) · kv_heads, the heads of the same
 // rows next to one another (they lie side by side in the dense buffers), block 256.
+// Four CTAs an SM (64 registers) rather than three: 32768 int8 rows of 8 heads
+// of 128 took 93 us against 117, 24000 e4m3 rows 59.5 against 62.3.
 template <typename T, int D, bool E4M3>
-__global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_append_block(KvCacheDev c, KvBatchDev b, RowsDev keys, RowsDev values, bool vector16) {
+__global__ void __launch_bounds__(ROW_WARPS * 32, 4) k_kv_append_block(KvCacheDev c, KvBatchDev b, RowsDev keys, RowsDev values, bool vector16) {
   constexpr int M = D / 16, AHEAD = sizeof(T) == 4 && D == 128 ? 1 : 2;
   const int lane = threadIdx.x & 31, h = blockIdx.x % c.kv_heads;
   const long long r0 = ((long long)(blockIdx.x / c.kv_heads) * ROW_WARPS + (threadIdx.x >> 5)) * BLOCK_ROWS;
@@ -532,8 +534,8 @@ static cudaError_t rows_launch(bool append, const KvCacheDev& c, const KvBatchDe
   // Blocks of rows where most of them can lie in one sequence and page, and
   // there are enough of them to fill the SMs. A row a warp against blocks, in us:
   //   one sequence, 4 heads of 64:   4096 rows 8.8 : 10.5 append, 5.5 : 5.4 read; 8192 13.5 : 11.6, 8.7 : 6.0
-  //   one sequence, 8 heads of 128:  2048 rows 12.2 : 14.3, 6.8 : 7.3; 4096 21.3 : 15.8, 11.1 : 8.2
-  //   32768 rows of 8 heads of 128, sequences of 8: 148 : 148, 95 : 71; of 16: 148 : 124, 92 : 50
+  //   one sequence, 8 heads of 128:  2048 rows 12.2 : 14.3, 6.8 : 7.3; 4096 21.3 : 17.4, 11.1 : 8.2
+  //   32768 rows of 8 heads of 128, sequences of 24: 147 : 102, 91 : 55
   if (b.max_rows >= BLOCK_ROWS && (long long)b.rows * c.kv_heads >= 148 * 16 * BLOCK_ROWS / 2) {
     // a lane's D / 16 elements in accesses of at most 16 bytes
     const bool vector16 = aligned_rows(keys, sizeof(T), D / 16) && aligned_rows(values, sizeof(T), D / 16);
