@@ -1,6 +1,6 @@
 // async.cuh — device-side building blocks that every kernel file shares:
-// packed f32 arithmetic, programmatic dependent launch, bounded mbarrier
-// waits and bulk copies.
+// packed f32 arithmetic, programmatic dependent launch, the cluster barrier's
+// halves, bounded mbarrier waits and bulk copies.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -40,6 +40,12 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 // (ld.global.cg), never through a possibly stale L1 line.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// The two halves of a cluster barrier. Distributed shared memory is usable once
+// every CTA of the cluster is known to run: an arrive where the kernel starts
+// and the wait before its first remote access cost next to nothing.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 // Bounded mbarrier waits: a wait that gives up returns false, and its caller
 // raises the device error flag and skips the work instead of hanging.

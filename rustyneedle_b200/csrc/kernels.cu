@@ -1383,8 +1383,6 @@ __host__ __device__ constexpr int att_wstride(int t_cap) { return t_cap / 4 + 2;
 // straight to shared memory, the key and value into the token's page slot,
 // which only this CTA reads in this pass.
 constexpr int ATT_ROWS = 0, ATT_CLUSTER = 1, ATT_LAST = 2;
-__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 template <int G, int EPI, bool HEADS, int W>
 __global__ void __launch_bounds__(W + 32, att_min_blocks(W)) k_attend(ModelDev md, LayerDev L, Work w, KvDev kv, int M, int layer, int t_cap) {

@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_verify(VerifyDev v, 
   constexpr int N = LogitRow<T>::N;
   __shared__ VerifyShared sh;
   cg::cluster_group cluster = cg::this_cluster();
+  cluster_arrive_relaxed();  // paired with the wait before the first remote store
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int s = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int words = (v.vocab + 31) / 32, pieces = LogitRow<T>::pieces(v.vocab), share = (pieces + ranks - 1) / ranks;
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_verify(VerifyDev v, 
   int turn = 0, kept = 0, best = 0;
   float top = -INFINITY;
   uint32_t unmasked = 0;  // rows of the round whose mask allows nothing
-  bool stop = false, redo = false;
+  bool stop = false, redo = false, alone = true;  // alone: the cluster's other CTAs may not run yet
   for (int i0 = 0; !stop;) {
     const int mine = warp / row_warps;
     // what the decisions need of the drafts, DRAFTS rows ahead: two dependent
@@ -398,6 +399,11 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_verify(VerifyDev v, 
         sum = m == -INFINITY ? 0.0f : __fmul_rn(sum, exp2_fast(__fmul_rn(__fadd_rn(m, -wm), step)));
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(FULL, sum, o));
+      }
+      if (alone) {
+        __syncwarp();
+        cluster_wait();  // every CTA of the cluster runs: its shared memory is usable
+        alone = false;
       }
       if (lane < ranks) {
         const int k = rank * WARPS + warp;

@@ -1,0 +1,42 @@
+"""Drafted decoding on the GPU at the limits of what its calls allow, against
+plain 64-bit forms."""
+
+import numpy as np
+import pytest
+
+from tests import serving_reference as ref
+from tests.test_gpu_serving import nb, torch, verify_inputs  # noqa: F401  (fixtures among them)
+
+pytestmark = pytest.mark.gpu
+
+
+def cuda_inputs(torch, x):  # noqa: F811
+    """verify_drafts' arguments for verify_inputs' numbers."""
+    put = lambda a, t: None if a is None else torch.tensor(np.ascontiguousarray(a), device="cuda:0").to(t)  # noqa: E731
+    args = [x["logits"], put(x["tokens"], torch.int32), put(x["accept"], torch.float32), put(x["sample"], torch.float32)]
+    more = {"draft_probabilities": put(x["q"], torch.float32), "temperature": x["temperature"]}
+    if x["mask"] is not None:
+        more["mask_bits"] = torch.tensor(x["mask"].view(np.int32), device="cuda:0")
+    return args, more
+
+
+def plain(x, counts=None):
+    return ref.verify(x["logits"].float().cpu().numpy(), x["tokens"], x["accept"], x["sample"], x["q"], counts, x["mask"], x["temperature"])
+
+
+def test_verify_many_clusters_on_several_streams(nb, torch):  # noqa: F811
+    """Clusters of one to eight blocks that start while others run: no block reaches into one that does not run yet."""
+    rng = np.random.default_rng(80)
+    jobs = []
+    for n, vocab, temperature in ((3, 9001, 1.0), (70, 3000, 1.0), (160, 2100, 0.0), (300, 1500, 0.9), (600, 300, 1.0)):
+        x = verify_inputs(rng, torch, n, 2, vocab, "bf16", temperature=temperature)
+        jobs.append((cuda_inputs(torch, x), plain(x), torch.cuda.Stream(), []))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for (args, more), _, stream, got in jobs:
+            with torch.cuda.stream(stream):
+                got.append(nb.verify_drafts(*args, **more))
+    torch.cuda.synchronize()
+    for _, want, _, got in jobs:
+        for tokens, accepted in got:
+            assert np.array_equal(tokens.cpu().numpy(), want[0]) and np.array_equal(accepted.cpu().numpy(), want[1])
