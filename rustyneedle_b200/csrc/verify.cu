@@ -202,7 +202,9 @@ __device__ __forceinline__ void take_pieces(const LogitRow<T>& row, int c, int s
     }
     st.any = true;
     const float high = fmaxf(to_f32(pair.x), to_f32(pair.y));
-    if (!(fminf(high, FLT_MAX) > st.m)) return;
+    // 64 NaNs leave a NaN, which is no maximum: it must not reach fminf, which
+    // would drop it for FLT_MAX
+    if (!(high > st.m) || st.m == FLT_MAX) return;
     st.m = fminf(high, FLT_MAX);  // no 16-bit value but +inf comes to FLT_MAX
 #pragma unroll
     for (int a = A - 1; a >= 0; --a) {

@@ -40,3 +40,36 @@ def test_verify_many_clusters_on_several_streams(nb, torch):  # noqa: F811
     for _, want, _, got in jobs:
         for tokens, accepted in got:
             assert np.array_equal(tokens.cpu().numpy(), want[0]) and np.array_equal(accepted.cpu().numpy(), want[1])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("n, vocab", [(200, 50257), (64, 32000), (8, 129283), (600, 17001)])
+def test_verify_greedy_passes_over_nan_in_long_rows(nb, torch, dtype, n, vocab):  # noqa: F811
+    """Rows long enough for several full steps of every thread: all of them NaN, NaN in all places of some threads, NaN
+    behind the maximum and before it, and infinities among them."""
+    from tests.test_gpu_serving import dtype_of
+
+    g = torch.Generator("cuda").manual_seed(vocab)
+    kinds, drafts, nan, inf = 8, 1, float("nan"), float("inf")
+    one = torch.randn(kinds, drafts + 1, vocab, generator=g, device="cuda:0")
+    ids = torch.arange(vocab, device="cuda:0")
+    lanes = (ids // 8 % 32 >= 5) & (ids // 8 % 32 <= 7)  # whole 16-byte pieces of one lane of every warp, however they start
+    one[0] = nan
+    one[1, :, lanes] = nan
+    one[2, :, 3] = 50.0
+    one[2, :, 9:] = nan
+    one[3, :, : vocab - 7] = nan
+    one[4, 0] = nan
+    one[4, 0, vocab // 2] = -3.0
+    one[5, :, vocab // 3 :] = nan
+    one[5, :, vocab // 5] = inf
+    one[6] = torch.where(lanes, nan, -inf)
+    one = one.to(dtype_of(torch, dtype))
+    clean = one.float().nan_to_num(nan=-inf, posinf=inf, neginf=-inf)
+    x = dict(logits=one, tokens=clean[:, :drafts].argmax(-1).cpu().numpy(), accept=None, sample=None, q=None, mask=None, temperature=0.0)
+    want = plain(x)
+    assert (want[0][[0, 6]] == -1).all()
+    of = torch.arange(n, device="cuda:0") % kinds
+    tokens, accepted = nb.verify_drafts(one[of].contiguous(), torch.tensor(x["tokens"], dtype=torch.int32, device="cuda:0")[of].contiguous(), None, None, temperature=0.0)
+    of = of.cpu().numpy()
+    assert np.array_equal(tokens.cpu().numpy(), want[0][of]) and np.array_equal(accepted.cpu().numpy(), want[1][of])
