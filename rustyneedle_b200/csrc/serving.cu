@@ -1,5 +1,6 @@
 // serving.cu — the C ABI of the drafted-decoding operators: the quantised
 // key/value cache, the shared-prefix attention and the verification of drafts.
+#include <algorithm>
 #include <climits>
 #include <string>
 
@@ -57,7 +58,9 @@ KvBatchDev batch_of(const nb_kv_batch& b) {
   KvBatchDev d;
   d.sequences = (int)b.sequences;
   d.rows = (int)b.rows;
-  d.max_rows = (int)b.max_rows;
+  // more rows than the batch has are no sequence's; the attention's tiles of a
+  // sequence, rows x query heads of a kv head, then stay within 32 bits
+  d.max_rows = (int)std::min(b.max_rows, b.rows);
   d.max_length = (int)b.max_length;
   d.page_stride = b.page_stride;
   d.row_start = b.row_start;
@@ -87,12 +90,12 @@ RowsDev rows_of(const nb_rows& r, const char* name, const nb_kv_batch& b, uint32
   return d;
 }
 
-void attend_sizes(const nb_kv_cache& c, const nb_kv_batch& b, uint32_t prefix_length, uint32_t heads) {
+void attend_sizes(const nb_kv_cache& c, const KvBatchDev& b, uint32_t prefix_length, uint32_t heads) {
   if (heads == 0 || heads % c.dev.kv_heads || heads / c.dev.kv_heads > (uint32_t)KV_MAX_GROUP)
     fail(NB_ERR_ARGUMENT, "heads must be a multiple of the cache's kv_heads, at most 64 for each");
   if (prefix_length > (1u << 30)) fail(NB_ERR_ARGUMENT, "prefix_length is above 2^30");
   const uint64_t group = heads / c.dev.kv_heads;
-  if ((uint64_t)b.rows * heads > (1ull << 30) || (uint64_t)b.sequences * ((b.max_rows * group + 15) / 16) > (uint64_t)INT_MAX)
+  if ((uint64_t)b.rows * heads > (1ull << 30) || (uint64_t)b.sequences * (((uint64_t)b.max_rows * group + 15) / 16) > (uint64_t)INT_MAX)
     fail(NB_ERR_ARGUMENT, "too many rows for one call");
 }
 
@@ -181,7 +184,7 @@ nb_status nb_kv_cache_attend_workspace(const nb_kv_cache* cache, const nb_kv_bat
   if (!cache || !batch || !bytes) return NB_ERR_ARGUMENT;
   return guard([&] {
     const KvBatchDev b = batch_of(*batch);
-    attend_sizes(*cache, *batch, prefix_length, heads);
+    attend_sizes(*cache, b, prefix_length, heads);
     *bytes = kv_attend_workspace(cache->dev, b, (int)prefix_length, (int)heads);
   });
 }
@@ -192,7 +195,7 @@ nb_status nb_kv_cache_attend(const nb_kv_cache* cache, const nb_kv_batch* batch,
   if (!cache || !batch || !query || !out) return NB_ERR_ARGUMENT;
   return guard([&] {
     const KvBatchDev b = batch_of(*batch);
-    attend_sizes(*cache, *batch, prefix_length, heads);
+    attend_sizes(*cache, b, prefix_length, heads);
     KvAttend a;
     a.query = rows_of(*query, "query", *batch, heads, cache->dev.dim, false);
     a.out = rows_of(*out, "out", *batch, heads, cache->dev.dim, true);

@@ -73,3 +73,12 @@ def test_verify_greedy_passes_over_nan_in_long_rows(nb, torch, dtype, n, vocab):
     tokens, accepted = nb.verify_drafts(one[of].contiguous(), torch.tensor(x["tokens"], dtype=torch.int32, device="cuda:0")[of].contiguous(), None, None, temperature=0.0)
     of = of.cpu().numpy()
     assert np.array_equal(tokens.cpu().numpy(), want[0][of]) and np.array_equal(accepted.cpu().numpy(), want[1][of])
+
+
+def test_attend_with_a_bound_of_rows_beyond_the_batch(nb, torch):  # noqa: F811
+    """max_rows may be as loose as the call allows: 2^26 rows of 64 heads are more (row, head) pairs than 31 bits count, and
+    the launch follows the batch's own rows instead."""
+    from tests.test_gpu_serving import attend_case
+
+    for seed, rows, lengths, prefix, heads, kv in ((81, [3, 1], [40, 70], 100, 64, 1), (82, [20, 0, 5], [20, 3, 90], 0, 64, 1), (83, [2], [2], 65, 8, 2)):
+        attend_case(nb, torch, seed, rows, lengths, prefix, heads, kv, 64, "int8", "bf16", bounds={"rows": sum(rows), "max_rows": 1 << 26})
