@@ -85,6 +85,13 @@ def _index_tensor(t, name: str, dims: int):
     return t
 
 
+def _counts(**values) -> None:
+    """Refuses what the C ABI's 32-bit counts do not hold; ctypes would drop the upper bits."""
+    for name, value in values.items():
+        if not 0 <= value < 1 << 32:
+            raise ValueError(f"{name} must lie in [0, 2^32)")
+
+
 class KvBatch:
     """The sequences of a call (nb_kv_batch): sequence b has the rows
     row_start[b] .. row_start[b + 1] of the dense tensors and lengths[b] cached
@@ -102,8 +109,7 @@ class KvBatch:
             raise ValueError("row_start holds one more entry than lengths, pages one row for each")
         if not row_start.device == lengths.device == pages.device:
             raise ValueError("row_start, lengths and pages must be on one GPU")
-        if min(rows, max_rows, max_length) < 0:
-            raise ValueError("rows, max_rows and max_length must not be negative")
+        _counts(rows=rows, max_rows=max_rows, max_length=max_length)
         self._kept = (row_start, lengths, pages)
         self.device = row_start.device.index
         self.rows = rows
@@ -119,6 +125,7 @@ class KvCache:
     def __init__(self, kv_heads: int, head_dim: int, pages: int, format: str = "int8", device: int = -1):
         if format not in FORMATS:
             raise ValueError(f"format must be one of {sorted(FORMATS)}")
+        _counts(kv_heads=kv_heads, head_dim=head_dim, pages=pages)
         L = _library()
         if device < 0 and _torch.cuda.is_available():
             device = _torch.cuda.current_device()
@@ -160,6 +167,7 @@ class KvCache:
         heads = query.shape[1] if query.dim() == 3 else 0
         q = self._rows(query, "query", batch.rows, heads)
         o = self._rows(out, "out", batch.rows, heads)
+        _counts(prefix_length=prefix_length)
         pages = None
         if prefix_length:
             _index_tensor(prefix_pages, "prefix_pages", 1)
