@@ -301,7 +301,7 @@ typedef enum nb_dtype { NB_F32 = 0, NB_F16 = 1, NB_BF16 = 2 } nb_dtype;
  *   magnitude), code = x / scale rounded to the nearest integer, halves to even.
  * NB_KV_E4M3: scale = the smallest power of two s with peak <= 448 s, code =
  *   x / s rounded to e4m3 (nearest, halves to even).
- * A row of zeros has scale 1. No scale is below 2^-60: rows of smaller numbers
+ * No scale is below 2^-60, which a row of zeros has: rows of smaller numbers
  * lose their low bits. A row with a NaN, an infinity or a
  * magnitude above 2^40 is held as NaN as a whole, and reads so. */
 typedef enum nb_kv_format { NB_KV_INT8 = 0, NB_KV_E4M3 = 1 } nb_kv_format;

@@ -10,7 +10,10 @@
 
 namespace nbk {
 
-// The row's scale and its reciprocal step; a row that cannot be held is NaN.
+// The row's scale and its reciprocal step; a row that cannot be held is NaN. A
+// row of zeros has the smallest scale: the attention's weights are normalised
+// by the largest exponent with the value scale in it, and a row that gives
+// nothing must not push those that give something out of f16.
 struct RowScale {
   float scale, inverse;
   bool held;
@@ -23,10 +26,6 @@ __device__ __forceinline__ RowScale row_scale(float peak, bool finite) {
   if (!r.held) {
     r.scale = __int_as_float(0x7fc00000);
     r.inverse = 0.0f;
-    return r;
-  }
-  if (peak == 0.0f) {
-    r.scale = r.inverse = 1.0f;
     return r;
   }
   if constexpr (E4M3) {
@@ -510,10 +509,11 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_read_block(KvCacheDev c, 
 }
 
 __global__ void k_kv_fill_scales(float* ks, float* vs, size_t n) {
-  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) ks[i] = vs[i] = 1.0f;
+  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) ks[i] = vs[i] = KV_SCALE_MIN;
 }
 
-// A fresh pool holds rows of zeros: no code of it is ever a NaN.
+// A fresh pool holds rows of zeros, at a row of zeros' scale: no code of it is
+// ever a NaN.
 cudaError_t kv_pool_clear(const KvCacheDev& c, cudaStream_t st) {
   const size_t blocks = (size_t)c.pages * c.kv_heads, bytes = blocks * KV_PAGE * c.dim;
   cudaError_t e = cudaMemsetAsync(c.k, 0, bytes, st);

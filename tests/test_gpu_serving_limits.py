@@ -82,3 +82,48 @@ def test_attend_with_a_bound_of_rows_beyond_the_batch(nb, torch):  # noqa: F811
 
     for seed, rows, lengths, prefix, heads, kv in ((81, [3, 1], [40, 70], 100, 64, 1), (82, [20, 0, 5], [20, 3, 90], 0, 64, 1), (83, [2], [2], 65, 8, 2)):
         attend_case(nb, torch, seed, rows, lengths, prefix, heads, kv, 64, "int8", "bf16", bounds={"rows": sum(rows), "max_rows": 1 << 26})
+
+
+@pytest.mark.parametrize("score", [10.0, 14.0, 25.0])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("bounds", [{}, {"rows": 8192, "max_rows": 2048, "max_length": 1 << 14}, {"rows": 4000, "max_rows": 150, "max_length": 1 << 17}])
+def test_attend_to_value_rows_of_zeros(nb, torch, kind, dim, score, bounds):  # noqa: F811
+    """A position that draws most of the attention and gives nothing, written as zeros or never written: the small rest is as
+    exact as without it. The bound is check_attend's, with its largest p vs over the rows that give something (a row of
+    zeros counts with the smallest scale, 2^-60)."""
+    from tests.test_gpu_serving import int32, make_batch, numbers, paged, random_rows
+
+    rng = np.random.default_rng(int(score) + dim)
+    kv, heads, prefix, rows, lengths = 2, 4, 300, [3, 40], [200, 230]
+    prefix_pages, table, pages = paged(rng, lengths, -(-prefix // 64))
+    total = prefix + sum(lengths)
+    keys = random_rows(rng, torch, total, kv, dim, torch.bfloat16) * 0.2
+    values = (0.02 + 0.004 * torch.randn(total, kv, dim, generator=torch.Generator("cuda").manual_seed(5), device="cuda:0")).to(torch.bfloat16)
+    query = random_rows(rng, torch, bounds.get("rows", sum(rows)), heads, dim, torch.bfloat16) * 0.2
+    # all other positions lie below the two rows of zeros, and those that were never written, by about `score`
+    query[:, :, 0] = dim**0.5
+    keys[:, :, 0] = -score
+    written = torch.ones(total, dtype=torch.bool)
+    zeros = [7, prefix + 20, prefix + lengths[0] + 64]
+    keys[zeros] = 0
+    values[zeros] = 0
+    fresh = slice(prefix + lengths[0], prefix + lengths[0] + 64)  # the second sequence's first page
+    keys[fresh], values[fresh], written[fresh] = 0, 0, False
+    cache = nb.KvCache(kv, dim, pages, format=kind, device=0)
+    cache.append(make_batch(nb, torch, [prefix], [prefix], prefix_pages[None]), keys[:prefix], values[:prefix])
+    own = written[prefix:].cuda()
+    cache.append(make_batch(nb, torch, [lengths[0], lengths[1] - 64], lengths, table), keys[prefix:][own], values[prefix:][own])
+    out = torch.full_like(query, 3.0)
+    cache.attend(make_batch(nb, torch, rows, lengths, table, **bounds), query, out, int32(torch, prefix_pages), prefix)
+    cache.check()
+    kc, ks = ref.quantise(numbers(keys), kind)
+    vc, vs = ref.quantise(numbers(values), kind)
+    vs = np.where((vc == 0).all(-1), 2.0**-60, vs)
+    n = sum(rows)
+    want, mass, size, least = ref.attend(numbers(query[:n]), kc * ks[..., None], vc, vs, rows, lengths, prefix, dim**-0.5)
+    weight = 2 * ((dim + 8) * 2.0**-23 * size + 2.0**-20)
+    eps = torch.finfo(torch.bfloat16).eps
+    bound = eps / 2 * np.abs(want) + mass * (2.0**-11 + weight + ((prefix + max(lengths)) / 8 + 16) * 2.0**-23) + 2.0**-33 * least
+    off = np.abs(numbers(out[:n]) - want)
+    assert (off <= bound).all(), float((off / np.abs(want)).max())
