@@ -136,6 +136,8 @@ class KvCache:
 
     def _rows(self, t, name: str, rows: int, heads: int) -> nb_rows:
         shape, stride = t.shape, t.stride()
+        if shape[:1] == (0,):  # torch gives a tensor of no rows any strides
+            stride = (heads * self.head_dim, self.head_dim, 1)
         if len(shape) != 3 or shape[0] < rows or shape[1] != heads or shape[2] != self.head_dim or stride[2] != 1:
             raise ValueError(f"{name} must be [at least {rows} rows][{heads}][{self.head_dim}] with a contiguous last dimension")
         if t.get_device() != self.device or t.dtype not in _DTYPES:
@@ -226,10 +228,10 @@ def verify_drafts(logits, draft_tokens, accept_uniforms, sample_uniforms, draft_
     the last; accepted [n] int32), written into the tensors given for them."""
     L = _lib or _library()
     torch = _torch
-    if logits.dim() != 3 or logits.stride(2) != 1 or logits.shape[1] < 1 or not logits.is_cuda or logits.dtype not in _DTYPES:
+    if logits.dim() != 3 or (logits.stride(2) != 1 and logits.shape[0]) or logits.shape[1] < 1 or not logits.is_cuda or logits.dtype not in _DTYPES:
         raise ValueError("logits must be a float CUDA tensor [sequences][drafts + 1][vocab] with a contiguous last dimension")
     n, rows, vocab = logits.shape
-    stride = logits.stride(1) if rows > 1 else logits.stride(0)
+    stride = vocab if n == 0 else logits.stride(1) if rows > 1 else logits.stride(0)
     if n > 1 and rows > 1 and logits.stride(0) != rows * stride:
         raise ValueError("the rows of logits must lie at one distance (a view of [sequences * (drafts + 1)] rows)")
     device, drafts = logits.device, rows - 1

@@ -127,3 +127,22 @@ def test_attend_to_value_rows_of_zeros(nb, torch, kind, dim, score, bounds):  # 
     bound = eps / 2 * np.abs(want) + mass * (2.0**-11 + weight + ((prefix + max(lengths)) / 8 + 16) * 2.0**-23) + 2.0**-33 * least
     off = np.abs(numbers(out[:n]) - want)
     assert (off <= bound).all(), float((off / np.abs(want)).max())
+
+
+def test_tensors_of_no_rows_whatever_their_strides(nb, torch):  # noqa: F811
+    """torch.tensor gives an empty array strides of zero."""
+    from tests.test_gpu_serving import make_batch
+
+    empty = lambda *shape: torch.tensor(np.zeros(shape), dtype=torch.bfloat16, device="cuda:0")  # noqa: E731
+    assert empty(0, 2, 64).stride() == (0, 0, 0)
+    cache = nb.KvCache(2, 64, 1, device=0)
+    for rows, lengths in (([], []), ([0, 0], [0, 3])):
+        batch = make_batch(nb, torch, rows, lengths, np.zeros((len(rows), 1), dtype=np.int32))
+        cache.append(batch, empty(0, 2, 64), empty(0, 2, 64))
+        cache.read(batch, empty(0, 2, 64), empty(0, 2, 64))
+        cache.attend(batch, empty(0, 4, 64), empty(0, 4, 64))
+    cache.check()
+    none = lambda *shape: torch.zeros(*shape, dtype=torch.float32, device="cuda:0")  # noqa: E731
+    for drafts in (0, 2):
+        tokens, accepted = nb.verify_drafts(empty(0, drafts + 1, 50), none(0, drafts).int(), none(0, drafts), none(0))
+        assert tokens.shape == (0, drafts + 1) and accepted.shape == (0,)
