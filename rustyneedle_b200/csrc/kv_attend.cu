@@ -597,7 +597,8 @@ static cudaError_t attend_launch(const AttendDev& d, const AttendPlan& p, cudaSt
 }
 
 cudaError_t kv_attend(const KvCacheDev& c, const KvBatchDev& b, const KvAttend& x, cudaStream_t st) {
-  if (b.sequences == 0 || b.rows == 0) return cudaSuccess;
+  if (b.rows == 0) return kv_check_spans(c, b, st);
+  if (b.sequences == 0) return cudaSuccess;
   const AttendPlan p = attend_plan(c, b, x.prefix, x.heads);
   AttendDev d;
   d.c = c;

@@ -128,10 +128,7 @@ __device__ __forceinline__ RowPlace place_of(const KvCacheDev& c, const KvBatchD
   const int lane = threadIdx.x & 31;
   const int s = sequence_of(b, row);
   const Span sp = span_of(b, s);
-  if (!sp.ok) {
-    if (lane == 0) atomicOr(c.error, KV_BAD_SEQUENCE);
-    return p;
-  }
+  if (!sp.ok) return p;  // check_spans reports it
   if (row < sp.first || row >= sp.first + sp.n) return p;
   const int position = sp.len - sp.n + (row - sp.first);
   const uint32_t page = b.pages[(size_t)s * b.page_stride + position / KV_PAGE];
@@ -145,10 +142,30 @@ __device__ __forceinline__ RowPlace place_of(const KvCacheDev& c, const KvBatchD
   return p;
 }
 
+// Reports the sequences that break their bounds, wherever their rows lie (a
+// sequence behind the batch's rows is met by none of them): a thread for each,
+// in blocks behind those that take the rows.
+__device__ __forceinline__ void check_spans(const KvCacheDev& c, const KvBatchDev& b, unsigned block) {
+  const long long s = (long long)block * (ROW_WARPS * 32) + threadIdx.x;
+  if (s < b.sequences && !span_of(b, (int)s).ok) atomicOr(c.error, KV_BAD_SEQUENCE);
+}
+
+__global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_check_spans(KvCacheDev c, KvBatchDev b) { check_spans(c, b, blockIdx.x); }
+
+static unsigned span_blocks(const KvBatchDev& b) { return (unsigned)((b.sequences + ROW_WARPS * 32 - 1) / (ROW_WARPS * 32)); }
+
+cudaError_t kv_check_spans(const KvCacheDev& c, const KvBatchDev& b, cudaStream_t st) {
+  if (b.sequences == 0) return cudaSuccess;
+  k_kv_check_spans<<<span_blocks(b), ROW_WARPS * 32, 0, st>>>(c, b);
+  return cudaGetLastError();
+}
+
 // A warp for `each` units of a row (a multiple of four, or all that there
-// are). grid ceil(rows · shares / 8), block 256.
+// are). grid row_blocks = ceil(rows · shares / 8), and those of check_spans;
+// block 256.
 template <typename T, int D, bool E4M3>
-__global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_append(KvCacheDev c, KvBatchDev b, RowsDev keys, RowsDev values, bool vector, int each, int shares) {
+__global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_append(KvCacheDev c, KvBatchDev b, RowsDev keys, RowsDev values, bool vector, int each, int shares, unsigned row_blocks) {
+  if (blockIdx.x >= row_blocks) return check_spans(c, b, blockIdx.x - row_blocks);
   constexpr int N = D / 32;
   const int lane = threadIdx.x & 31;
   const long long item = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
@@ -199,7 +216,8 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_append(KvCacheDev c, KvBa
 
 // The same units, read back: code · scale, rounded once.
 template <typename T, int D, bool E4M3>
-__global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_read(KvCacheDev c, KvBatchDev b, RowsDev keys, RowsDev values, bool vector, int each, int shares) {
+__global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_read(KvCacheDev c, KvBatchDev b, RowsDev keys, RowsDev values, bool vector, int each, int shares, unsigned row_blocks) {
+  if (blockIdx.x >= row_blocks) return check_spans(c, b, blockIdx.x - row_blocks);
   constexpr int N = D / 32;
   const int lane = threadIdx.x & 31;
   const long long item = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
@@ -263,9 +281,7 @@ __device__ __forceinline__ bool block_places(const KvCacheDev& c, const KvBatchD
       }
     }
     const Span sp = span_of(b, s);
-    if (!sp.ok) {
-      atomicOr(c.error, KV_BAD_SEQUENCE);
-    } else if (row >= sp.first && row < sp.first + sp.n) {
+    if (sp.ok && row >= sp.first && row < sp.first + sp.n) {
       const int position = sp.len - sp.n + (row - sp.first);
       const uint32_t page = b.pages[(size_t)s * b.page_stride + position / KV_PAGE];
       p.ok = page < c.pages;
@@ -335,12 +351,14 @@ __device__ __forceinline__ uint32_t peak_bits(const float (&x)[N]) {
 }
 
 // A half warp a row: lanes 0 - 15 rows 0 - 7, lanes 16 - 31 rows 8 - 15, D / 16
-// dimensions a lane. grid ceil(rows / 16 / 8) · kv_heads, the heads of the same
-// rows next to one another (they lie side by side in the dense buffers), block 256.
+// dimensions a lane. grid row_blocks = ceil(rows / 16 / 8) · kv_heads, the heads of
+// the same rows next to one another (they lie side by side in the dense buffers),
+// and those of check_spans; block 256.
 // Four CTAs an SM (64 registers) rather than three: 32768 int8 rows of 8 heads
 // of 128 took 93 us against 117, 24000 e4m3 rows 59.5 against 62.3.
 template <typename T, int D, bool E4M3>
-__global__ void __launch_bounds__(ROW_WARPS * 32, 4) k_kv_append_block(KvCacheDev c, KvBatchDev b, RowsDev keys, RowsDev values, bool vector16) {
+__global__ void __launch_bounds__(ROW_WARPS * 32, 4) k_kv_append_block(KvCacheDev c, KvBatchDev b, RowsDev keys, RowsDev values, bool vector16, unsigned row_blocks) {
+  if (blockIdx.x >= row_blocks) return check_spans(c, b, blockIdx.x - row_blocks);
   constexpr int M = D / 16, AHEAD = sizeof(T) == 4 && D == 128 ? 1 : 2;
   const int lane = threadIdx.x & 31, h = blockIdx.x % c.kv_heads;
   const long long r0 = ((long long)(blockIdx.x / c.kv_heads) * ROW_WARPS + (threadIdx.x >> 5)) * BLOCK_ROWS;
@@ -437,7 +455,8 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, 4) k_kv_append_block(KvCacheDe
 }
 
 template <typename T, int D, bool E4M3>
-__global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_read_block(KvCacheDev c, KvBatchDev b, RowsDev keys, RowsDev values, bool vector16) {
+__global__ void __launch_bounds__(ROW_WARPS * 32) k_kv_read_block(KvCacheDev c, KvBatchDev b, RowsDev keys, RowsDev values, bool vector16, unsigned row_blocks) {
+  if (blockIdx.x >= row_blocks) return check_spans(c, b, blockIdx.x - row_blocks);
   constexpr int M = D / 16;
   const int lane = threadIdx.x & 31, h = blockIdx.x % c.kv_heads;
   const long long r0 = ((long long)(blockIdx.x / c.kv_heads) * ROW_WARPS + (threadIdx.x >> 5)) * BLOCK_ROWS;
@@ -541,9 +560,9 @@ static cudaError_t rows_launch(bool append, const KvCacheDev& c, const KvBatchDe
     const bool vector16 = aligned_rows(keys, sizeof(T), D / 16) && aligned_rows(values, sizeof(T), D / 16);
     const unsigned blocks = (unsigned)((b.rows + BLOCK_ROWS * ROW_WARPS - 1) / (BLOCK_ROWS * ROW_WARPS)) * c.kv_heads;
     if (append)
-      k_kv_append_block<T, D, E4M3><<<blocks, ROW_WARPS * 32, 0, st>>>(c, b, keys, values, vector16);
+      k_kv_append_block<T, D, E4M3><<<blocks + span_blocks(b), ROW_WARPS * 32, 0, st>>>(c, b, keys, values, vector16, blocks);
     else
-      k_kv_read_block<T, D, E4M3><<<blocks, ROW_WARPS * 32, 0, st>>>(c, b, keys, values, vector16);
+      k_kv_read_block<T, D, E4M3><<<blocks + span_blocks(b), ROW_WARPS * 32, 0, st>>>(c, b, keys, values, vector16, blocks);
     return cudaGetLastError();
   }
   // all units of a row for a warp, unless that leaves SMs short of warps (16
@@ -555,9 +574,9 @@ static cudaError_t rows_launch(bool append, const KvCacheDev& c, const KvBatchDe
   const int shares = (units + each - 1) / each;
   const unsigned grid = (unsigned)(((long long)b.rows * shares + ROW_WARPS - 1) / ROW_WARPS);
   if (append)
-    k_kv_append<T, D, E4M3><<<grid, ROW_WARPS * 32, 0, st>>>(c, b, keys, values, vector, each, shares);
+    k_kv_append<T, D, E4M3><<<grid + span_blocks(b), ROW_WARPS * 32, 0, st>>>(c, b, keys, values, vector, each, shares, grid);
   else
-    k_kv_read<T, D, E4M3><<<grid, ROW_WARPS * 32, 0, st>>>(c, b, keys, values, vector, each, shares);
+    k_kv_read<T, D, E4M3><<<grid + span_blocks(b), ROW_WARPS * 32, 0, st>>>(c, b, keys, values, vector, each, shares, grid);
   return cudaGetLastError();
 }
 
@@ -569,7 +588,8 @@ static cudaError_t rows_launch(bool append, const KvCacheDev& c, const KvBatchDe
 }
 
 static cudaError_t rows_launch(bool append, const KvCacheDev& c, const KvBatchDev& b, const RowsDev& keys, const RowsDev& values, cudaStream_t st) {
-  if (b.sequences == 0 || b.rows == 0) return cudaSuccess;
+  if (b.rows == 0) return kv_check_spans(c, b, st);
+  if (b.sequences == 0) return cudaSuccess;
   if (keys.dtype == DTYPE_F32) return rows_launch<float>(append, c, b, keys, values, st);
   if (keys.dtype == DTYPE_F16) return rows_launch<__half>(append, c, b, keys, values, st);
   return rows_launch<__nv_bfloat16>(append, c, b, keys, values, st);

@@ -146,3 +146,50 @@ def test_tensors_of_no_rows_whatever_their_strides(nb, torch):  # noqa: F811
     for drafts in (0, 2):
         tokens, accepted = nb.verify_drafts(empty(0, drafts + 1, 50), none(0, drafts).int(), none(0, drafts), none(0))
         assert tokens.shape == (0, drafts + 1) and accepted.shape == (0,)
+
+
+OUT_OF_BOUNDS = [  # rows, lengths, bounds: each with one sequence that breaks a bound without a row of it below the batch's rows
+    ([3, 3], [3, 3], {"rows": 3}), ([3, 0, 2], [3, 200, 2], {"max_length": 100}), ([3, 0, 2], [3, 65, 2], {"max_length": 1000}),
+    ([2, 0], [2, -1], {}), ([4, 4], [4, 4], {"rows": 0}), ([0, 0], [5, 90], {"max_length": 64}), ([5] * 300 + [2], [5] * 301, {"rows": 1500}),
+    ([2000, 7], [2000, 7], {"rows": 2000}),  # by blocks of 16 rows
+]
+
+
+@pytest.mark.parametrize("call", ["append", "read", "attend"])
+@pytest.mark.parametrize("case", range(len(OUT_OF_BOUNDS)))
+def test_sequences_that_break_a_bound_are_reported_by_every_call(nb, torch, call, case):  # noqa: F811
+    from tests.test_gpu_serving import held, make_batch, numbers, random_rows
+
+    rows, lengths, more = OUT_OF_BOUNDS[case]
+    rng = np.random.default_rng(90 + case)
+    n, kv, dim = sum(rows), 8, 64
+    pages = [max(1, -(-t // 64)) for t in lengths]
+    stride = 1 if max(lengths) < 1000 else max(pages)
+    table = np.arange(len(rows) * stride).reshape(len(rows), stride)
+    cache = nb.KvCache(kv, dim, table.size, device=0)
+    keys, values = (random_rows(rng, torch, n, kv, dim, torch.float32) for _ in range(2))
+    good = make_batch(nb, torch, rows, [max(r, min(t, 64)) if stride == 1 else t for r, t in zip(rows, lengths)], table)
+    cache.append(good, keys, values)
+    cache.check()
+    batch = make_batch(nb, torch, rows, lengths, table, **more)
+    out = [torch.full_like(keys, 9.0) for _ in range(2)]
+    if call == "append":
+        cache.append(batch, -keys, -values)
+    elif call == "read":
+        cache.read(batch, *out)
+    else:
+        cache.attend(batch, keys.bfloat16(), torch.full_like(keys, 9.0, dtype=torch.bfloat16))
+    with pytest.raises(nb.NeedleError) as e:
+        cache.check()
+    assert e.value.status == -4 and "sequence" in e.value.message
+    cache.check()  # cleared
+    if call == "append":
+        cache.read(good, *out)
+        cache.check()
+        keys = -keys
+    if call != "attend":  # the others are served
+        first = rows[0] if batch.rows else 0
+        assert np.array_equal(numbers(out[0][:first]), held(numbers(keys[:first]), "int8", torch.float32, torch))
+        left = out[0][batch.rows :]
+        want = held(numbers(-keys[batch.rows :]), "int8", torch.float32, torch) if call == "append" else np.full(left.shape, 9.0)
+        assert np.array_equal(numbers(left), want)
