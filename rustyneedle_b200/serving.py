@@ -136,12 +136,13 @@ class KvCache:
 
     def _rows(self, t, name: str, rows: int, heads: int) -> nb_rows:
         shape, stride = t.shape, t.stride()
-        if shape[:1] == (0,):  # torch gives a tensor of no rows any strides
-            stride = (heads * self.head_dim, self.head_dim, 1)
-        if len(shape) != 3 or shape[0] < rows or shape[1] != heads or shape[2] != self.head_dim or stride[2] != 1:
+        have = shape[0] if len(shape) == 3 else -1
+        if have < rows or shape[1] != heads or shape[2] != self.head_dim or (stride[2] != 1 and have):
             raise ValueError(f"{name} must be [at least {rows} rows][{heads}][{self.head_dim}] with a contiguous last dimension")
         if t.get_device() != self.device or t.dtype not in _DTYPES:
             raise ValueError(f"{name} must be a float32, float16 or bfloat16 tensor on cuda:{self.device}")
+        if not have:  # torch gives a tensor of no rows any strides
+            stride = (heads * self.head_dim, self.head_dim)
         return nb_rows(t.data_ptr(), _DTYPES[t.dtype], stride[0], stride[1])
 
     def _batch(self, batch: KvBatch):
@@ -169,7 +170,8 @@ class KvCache:
         heads = query.shape[1] if query.dim() == 3 else 0
         q = self._rows(query, "query", batch.rows, heads)
         o = self._rows(out, "out", batch.rows, heads)
-        _counts(prefix_length=prefix_length)
+        if not 0 <= prefix_length < 1 << 32:
+            raise ValueError("prefix_length must lie in [0, 2^32)")
         pages = None
         if prefix_length:
             _index_tensor(prefix_pages, "prefix_pages", 1)
