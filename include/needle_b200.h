@@ -421,8 +421,9 @@ typedef struct nb_verify {
  * accepted[b] is the number of accepted drafts; tokens[b] are these, the drawn
  * token, then UINT32_MAX. A NaN logit counts as -inf and +inf as the largest
  * float; a row with nothing left but -inf accepts nothing and draws
- * UINT32_MAX. A drafted id outside the vocabulary is never accepted. The
- * probabilities and running sums that decide a draw are formed in 64 bits. */
+ * UINT32_MAX. A drafted id outside the vocabulary is never accepted. What
+ * decides is formed in 64 bits, wherever 32 leave it open: an acceptance with
+ * the probability itself, a draw with running sums of weights within 1e-11. */
 nb_status nb_verify_drafts(int32_t device, const nb_verify* verify, void* stream);
 
 #ifdef __cplusplus

@@ -13,7 +13,9 @@
 // come to the same decision. The one row that a token is drawn from is read
 // once or twice more, from L2, with exponentials and running sums in f64: f32
 // sums over a large vocabulary would put some draws on the wrong side of a
-// border.
+// border. So they would some acceptances: where u · q and p are closer than the
+// f32 sum's error (about one draft in 10000), the round is gone through again
+// with that row's sum in f64.
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -45,7 +47,7 @@ struct LogitRow {
     head = min(v, (int)((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T)));
   }
   // the same for every row of a launch: pieces that any alignment needs
-  __device__ __forceinline__ static int pieces(int v) { return v / N + 2; }
+  __host__ __device__ static int pieces(int v) { return v / N + 2; }
   __device__ __forceinline__ int start(int piece) const { return head + (piece - 1) * N; }
   // pieces [1, whole_end()) lie whole within the row
   __device__ __forceinline__ int whole_end() const { return (vocab - head) / N + 1; }
@@ -165,6 +167,17 @@ struct RowStats {
   bool any = false;  // an id is allowed
 };
 constexpr float BASE_MOST = 32768.0f;  // beyond it, base is too coarse for the product
+
+// Twice the largest relative error of a row's sum, in units of 2^-24, where a
+// thread adds up `batches` batches of at most 64 weights. A weight 2^-a comes
+// from three roundings of a (the step, the product, the difference) and ex2,
+// within 2^-22; the mean of a over the weights is at most log2 vocab <= 24, so
+// that is 24 · 3 · ln 2 + 4 = 54, and as much again where a thread's sum comes
+// to its warp's maximum and a warp's to the row's. Adding up: 64 for a batch, 8
+// for the shift and the warp, and for every batch 8 for the sum's own rescaling
+// and addition. In all 3 · 54 + 72 < 256, and 8 a batch.
+static double sum_slack(int batches) { return (512 + 16 * batches) * 0x1p-24; }
+enum Verdict : int { REJECTED, ACCEPTED, UNSURE };
 
 // The pieces c, c + stride, .. below `end`, A of them at once so that their
 // loads overlap and the maximum is looked at once for all. CLEAN: they are
@@ -319,12 +332,19 @@ struct VerifyShared {
   uint32_t draft[DRAFTS];
   float draft_logit[DRAFTS], draft_q[DRAFTS], uniform[DRAFTS];
   int draft_allowed[DRAFTS];
-  bool row_accept[VERIFY_MAX_ROWS];
+  Verdict row_verdict[VERIFY_MAX_ROWS];
   double table[EXP_ENTRIES * EXP_COPIES];
 };
 
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(FULL, x, o);
+  return x;
+}
+
+// slack: sum_slack of the launch's rows
 template <typename T, bool GREEDY, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_verify(VerifyDev v, int at_once) {
+__global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_verify(VerifyDev v, int at_once, double slack) {
   constexpr int N = LogitRow<T>::N;
   __shared__ VerifyShared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -347,6 +367,7 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_verify(VerifyDev v, 
   int turn = 0, kept = 0, best = 0;
   float top = -INFINITY;
   uint32_t unmasked = 0;  // rows of the round whose mask allows nothing
+  uint32_t exact = 0;     // rows of the round whose sums are formed in f64
   bool stop = false, redo = false, alone = true;  // alone: the cluster's other CTAs may not run yet
   for (int i0 = 0; !stop;) {
     const int mine = warp / row_warps;
@@ -371,7 +392,10 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_verify(VerifyDev v, 
     {
       const int i = i0 + mine;
       RowStats<GREEDY> st;
-      if (i <= drafts) {
+      if (!GREEDY && exact >> mine & 1) {
+        st.m = sh.row_top[mine];  // of the pass before
+        st.any = true;
+      } else if (i <= drafts) {
         const LogitRow<T> row = row_of(i, unmasked >> mine & 1);
         const int stride = row_warps * 32;
         int c = lo + (warp % row_warps) * 32 + lane;
@@ -407,6 +431,16 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_verify(VerifyDev v, 
         cluster_wait();  // every CTA of the cluster runs: its shared memory is usable
         alone = false;
       }
+      if (!GREEDY && __builtin_expect(exact >> mine & 1, 0)) {
+        const LogitRow<T> row = row_of(i, unmasked >> mine & 1);
+        const int threads = row_warps * 32;
+        double precise = 0.0;
+#pragma unroll 1
+        for (int id = rank * threads + tid % threads; id < v.vocab; id += ranks * threads)
+          if (row.permits(id)) precise += exp(((double)tame(to_f32(row.p[id])) - (double)m) * inverse);
+        precise = warp_sum(precise);
+        if (lane < ranks) *cluster.map_shared_rank(&sh.draw[turn][rank * WARPS + warp], lane) = precise;
+      }
       if (lane < ranks) {
         const int k = rank * WARPS + warp;
         *cluster.map_shared_rank(&sh.top[turn][k], lane) = wm;
@@ -428,49 +462,61 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_verify(VerifyDev v, 
       for (int k = lane; k < count; k += 32) {
         const float t = sh.top[turn][entry(k)];
         if (!GREEDY || t == m) at = min(at, sh.at[turn][entry(k)]);
-        if (!GREEDY && t != -INFINITY) total += (double)sh.sum[turn][entry(k)] * (double)exp2f(__fmul_rn(__fadd_rn(t, -m), step));
+        if (!GREEDY && exact >> warp & 1)
+          total += sh.draw[turn][entry(k)];
+        else if (!GREEDY && t != -INFINITY)
+          total += (double)sh.sum[turn][entry(k)] * (double)exp2f(__fmul_rn(__fadd_rn(t, -m), step));
       }
       at = __reduce_min_sync(FULL, at);
-      bool accept = false;
+      Verdict verdict = REJECTED;
       if (i < drafts) {
         if (GREEDY) {
-          accept = sh.draft[i % DRAFTS] == (uint32_t)at;
+          verdict = sh.draft[i % DRAFTS] == (uint32_t)at ? ACCEPTED : REJECTED;
         } else {
 #pragma unroll
           for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
           const int k = i % DRAFTS;
           const float x = sh.draft_logit[k];
-          if (x != -INFINITY && (sh.draft_allowed[k] || (unmasked >> warp & 1)))
-            accept = (double)sh.uniform[k] * (double)sh.draft_q[k] * total < exp(((double)x - (double)m) * inverse);
+          if (x != -INFINITY && (sh.draft_allowed[k] || (unmasked >> warp & 1))) {
+            const double left = (double)sh.uniform[k] * (double)sh.draft_q[k] * total, right = exp(((double)x - (double)m) * inverse);
+            const bool near = fabs(left - right) < slack * right && !(exact >> warp & 1);
+            verdict = near ? UNSURE : left < right ? ACCEPTED : REJECTED;  // NaN: rejected
+          }
         }
       }
       if (lane == 0) {
         sh.row_top[warp] = m;
         sh.row_at[warp] = at;
-        sh.row_accept[warp] = accept;
+        sh.row_verdict[warp] = verdict;
       }
     }
     __syncthreads();
-    uint32_t again = 0;
+    bool again = false;
     for (int r = 0; r < at_once && !stop; ++r) {
       if (sh.row_at[r] == INT_MAX && !(unmasked >> r & 1)) {
-        again = 1u << r;  // the mask allows nothing: all ids
+        unmasked |= 1u << r;  // the mask allows nothing: all ids
+        again = true;
+        break;
+      }
+      const Verdict verdict = sh.row_verdict[r];
+      if (!GREEDY && verdict == UNSURE) {
+        exact |= 1u << r;
+        again = true;
         break;
       }
       top = sh.row_top[r];
       best = sh.row_at[r];
-      stop = top == -INFINITY || !sh.row_accept[r];
+      stop = top == -INFINITY || verdict != ACCEPTED;
       if (!stop) ++kept;
     }
     // the other set next: a slower CTA may still read this one
     turn ^= 1;
-    redo = again != 0;
+    redo = again;
     if (again) {
-      kept = i0;  // the round once more, with that row unmasked
-      unmasked |= again;
+      kept = i0;  // the round once more, with that row unmasked or exact
     } else if (!stop) {
       i0 += at_once;
-      unmasked = 0;
+      unmasked = exact = 0;
     } else {
       unmasked = unmasked >> (kept - i0) & 1;
     }
@@ -572,11 +618,6 @@ __global__ void __launch_bounds__(WARPS * 32, 32 / WARPS) k_verify(VerifyDev v, 
   };
   // a run is gone through 32 pieces a step, its steps in DRAW_GROUPS groups
   const int steps = (run + 31) / 32, group = (steps + DRAW_GROUPS - 1) / DRAW_GROUPS * 32;
-  auto warp_sum = [](double x) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(FULL, x, o);
-    return x;
-  };
   auto all_sums = [&](bool less) {  // sh.group[turn] and, in every CTA, sh.draw[turn] = every warp's sum
     double whole = 0.0;
     Piece<N> next;
@@ -721,8 +762,10 @@ static cudaError_t verify_launch(const VerifyDev& v, int ranks, int warps, int a
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (v.temperature == 0.0f) return cudaLaunchKernelEx(&cfg, warps == 16 ? k_verify<T, true, 16> : k_verify<T, true, 8>, v, at_once);
-  return cudaLaunchKernelEx(&cfg, warps == 16 ? k_verify<T, false, 16> : k_verify<T, false, 8>, v, at_once);
+  // a CTA's pieces over a row's threads, 4 pieces a batch at least, and the row's two ends
+  const double slack = sum_slack((LogitRow<T>::pieces(v.vocab) / ranks + 1) / (warps / at_once * 32 * 4) + 4);
+  if (v.temperature == 0.0f) return cudaLaunchKernelEx(&cfg, warps == 16 ? k_verify<T, true, 16> : k_verify<T, true, 8>, v, at_once, slack);
+  return cudaLaunchKernelEx(&cfg, warps == 16 ? k_verify<T, false, 16> : k_verify<T, false, 8>, v, at_once, slack);
 }
 
 cudaError_t verify_drafts(const VerifyDev& v, cudaStream_t st) {

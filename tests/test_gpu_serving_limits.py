@@ -193,3 +193,36 @@ def test_sequences_that_break_a_bound_are_reported_by_every_call(nb, torch, call
         left = out[0][batch.rows :]
         want = held(numbers(-keys[batch.rows :]), "int8", torch.float32, torch) if call == "append" else np.full(left.shape, 9.0)
         assert np.array_equal(numbers(left), want)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("n, drafts, vocab, masked, given, temperature", [
+    (60, 9, 20011, False, False, 1.0), (200, 9, 8192, True, True, 0.8), (6, 9, 129283, False, True, 1.0), (400, 9, 5000, False, True, 1.3),
+    (2, 9, 300007, False, False, 1.0), (30, 9, 300, True, False, 1.0), (20, 70, 500, True, True, 1.0), (20, 130, 90, False, True, 2.0)])
+def test_verify_accept_numbers_next_to_their_border(nb, torch, dtype, n, drafts, vocab, masked, given, temperature):  # noqa: F811
+    """The accept number is a step of f32 below p / q or above it, so that only a 64-bit p decides rightly: runs of drafts
+    below it, then one above."""
+    rng = np.random.default_rng(vocab)
+    # the call takes an f32: 0.8 is 1.5e-8 above, which moves a p of e^-30 by 6e-7, ten steps of an accept number
+    temperature = float(np.float32(temperature))
+    x = verify_inputs(rng, torch, n, drafts, vocab, dtype, masked, given, temperature, noise=0.3)
+    logits = x["logits"].double().cpu().numpy()
+    for b in range(n):
+        for i in range(drafts):
+            l = logits[b, i]
+            if masked and ref.unpack(x["mask"][b, i], vocab).any():
+                l = np.where(ref.unpack(x["mask"][b, i], vocab), l, -np.inf)
+            p = np.exp((l - l.max()) / temperature)
+            p /= p.sum()
+            d = int(x["tokens"][b, i])
+            border = p[d] / (float(x["q"][b, i, d]) if given else 1.0)
+            u = np.float32(border)
+            above = b > 0 and (rng.random() < 1.5 / drafts or b == 1)
+            if (float(u) > border) != above:
+                u = np.nextafter(u, np.float32(np.inf if above else -np.inf))
+            x["accept"][b, i] = u
+    (args, more), want = cuda_inputs(torch, x), plain(x)
+    tokens, accepted = nb.verify_drafts(*args, **more)
+    assert want[1][0] == drafts and want[1][1] == 0
+    assert np.array_equal(accepted.cpu().numpy(), want[1]), (accepted.cpu().numpy() != want[1]).mean()
+    assert np.array_equal(tokens.cpu().numpy(), want[0])
