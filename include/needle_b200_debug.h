@@ -51,6 +51,14 @@ nb_status nb_debug_product(int device, uint32_t bits, const uint8_t* packed, con
  * sessions and models are not affected. No reference counterpart. */
 nb_status nb_debug_expire_waits(nb_model* model, uint32_t count);
 
+/* The same for the shared-prefix attention: while `on` is not 0, the first block
+ * of every attention launch of a call on `cache` gives up a short bounded wait on
+ * a barrier that nobody completes (in the warp that issues the matrix
+ * instructions where a block has one: the waits of its other warps then run out
+ * too), lets its copies and matrix instructions end and returns, its rows NaN;
+ * nb_kv_cache_check then reports NB_ERR_TIMEOUT. No reference counterpart. */
+nb_status nb_debug_expire_attention(nb_kv_cache* cache, uint32_t on);
+
 /* A plain streaming read of a `bytes`-long device buffer (a multiple of 16)
  * on device `device`, through L2 with 16-byte loads, four 512-thread CTAs per
  * SM, `passes` (1-4096) reads of the whole buffer per launch: *ms_per_read

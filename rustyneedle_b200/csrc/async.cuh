@@ -67,6 +67,14 @@ __device__ __forceinline__ bool mbar_wait_polls(uint32_t bar, uint32_t phase, ui
   }
   return false;
 }
+// The same, given up also once another thread of the block has.
+__device__ __forceinline__ bool mbar_wait_polls(uint32_t bar, uint32_t phase, uint32_t polls, const int* failed) {
+  for (uint32_t i = 0; i < polls; i += 64) {
+    if (mbar_wait_polls(bar, phase, 64)) return true;
+    if (*static_cast<const volatile int*>(failed)) return false;
+  }
+  return false;
+}
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t phase) {
   for (uint32_t i = 0; i < MBAR_WAIT_LIMIT; ++i) {
     uint32_t done;

@@ -64,7 +64,7 @@ struct AttSmem {
     float o[ATT_WARPS][16][D + 4];  // once every copy has landed and been used
   };
   float2 ml[ATT_WARPS][16];
-  uint64_t full[ATT_WARPS][ATT_STAGES];
+  uint64_t full[ATT_WARPS][ATT_STAGES], never;
   int failed;
 };
 
@@ -135,9 +135,9 @@ struct Joined {
 };
 
 // FUSED (tails of one part): the prefix's parts are joined in, and the rows
-// written out.
+// written out. Three blocks an SM at D = 128, which is what their rings allow.
 template <int D, bool BF16, bool E4M3, bool PREFIX>
-__global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool fused) {
+__global__ void __launch_bounds__(ATT_WARPS * 32, D == 64 ? 4 : 3) k_kv_attend(AttendDev a, bool fused) {
   constexpr int SEG = D / 64, STEPS = D / 16, NT = D / 8;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   AttSmem<D>& sm = *reinterpret_cast<AttSmem<D>*>(smem_raw);
@@ -174,8 +174,11 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
   const int groups = max(0, (k1 - k0 + 31) / 32), count = max(0, (groups - warp + ATT_WARPS - 1) / ATT_WARPS);
   if (lane == 0)
     for (int i = 0; i < ATT_STAGES; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&sm.full[warp][i])) : "memory");
+  if (threadIdx.x == 0) {
+    sm.failed = 0;
+    if (a.c.expire) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&sm.never)) : "memory");
+  }
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  if (threadIdx.x == 0) sm.failed = 0;
   // the pages of the next 32 groups, one a lane
   uint32_t held = 0;
   int held_from = -32;
@@ -248,9 +251,11 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
   float o[NT][4] = {};
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   bool fine = true;
-  for (int i = 0; i < count; ++i) {
+  const int done = count > 0 && warp == 0 && expires(a.c) ? count - 1 : count;  // a test's wait runs out before the last group
+  int i = 0;
+  for (; i < done; ++i) {
     const int kb = k0 + 32 * (warp + ATT_WARPS * i);
-    fine = fine && __all_sync(FULL, mbar_wait_polls(smem_u32(&sm.full[warp][i % ATT_STAGES]), (i / ATT_STAGES) & 1, 1u << 18));
+    fine = __all_sync(FULL, mbar_wait_polls(smem_u32(&sm.full[warp][i % ATT_STAGES]), (i / ATT_STAGES) & 1, ATTEND_POLLS));
     if (!fine) break;
     const AttStage<D>& stage = sm.ring[warp][i % ATT_STAGES];
     if (!(bad >> (i & 31) & 1)) {
@@ -351,10 +356,11 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
     __syncwarp();
     if (i + ATT_STAGES < count) ask(i + ATT_STAGES);
   }
-  if (!fine && lane == 0) {  // what was asked for lands before the block ends
+  if (done < count) fine = __all_sync(FULL, mbar_wait_polls(smem_u32(&sm.never), 0, EXPIRE_POLLS));
+  if (!fine && lane == 0) {  // what was asked for, group i and those behind it, lands before the block ends
     sm.failed = 1;
     atomicOr(a.c.error, KV_WAIT_FAILED);
-    for (int i = 0; i < min(count, ATT_STAGES); ++i) mbar_wait_polls(smem_u32(&sm.full[warp][i]), 1, 1u << 18), mbar_wait_polls(smem_u32(&sm.full[warp][i]), 0, 1u << 18);
+    for (int j = i; j < min(count, i + ATT_STAGES); ++j) mbar_wait_polls(smem_u32(&sm.full[warp][j % ATT_STAGES]), (j / ATT_STAGES) & 1, ATTEND_POLLS);
   }
 
   // join the four warps, the ring's memory holding their accumulators
@@ -371,7 +377,6 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
     for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(&sm.o[warp][g + 8 * half][n * 8 + 2 * c]) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
   pdl_wait();  // the prefix's parts are complete (and whatever the launch before wrote)
   __syncthreads();
-  if (sm.failed) return;
   const int index = PREFIX ? part : a.prefix_parts + part;
   const size_t stride = (size_t)a.b.rows * a.heads;
   for (int x = threadIdx.x; x < 16 * D / 4; x += ATT_WARPS * 32) {
@@ -388,6 +393,7 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) k_kv_attend(AttendDev a, bool 
       v[w] = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
     }
     sum.add(ml, v);
+    if (sm.failed) sum.sum = NAN;  // and so is what it is joined into
     if (!fused) {
       const size_t at = index * stride + unit;
       *reinterpret_cast<float4*>(a.part_o + at * D + d) = make_float4(sum.y[0], sum.y[1], sum.y[2], sum.y[3]);

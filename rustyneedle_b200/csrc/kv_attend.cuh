@@ -6,6 +6,12 @@
 namespace nbk {
 
 constexpr float HEADROOM = 8.0f;
+
+// Every wait here is for work of microseconds; a poll that finds nothing takes
+// 4 us, so one gives up after a quarter of a second. That ends its block, whose
+// rows become NaN, and the report word says so.
+constexpr uint32_t ATTEND_POLLS = 1u << 16, EXPIRE_POLLS = 1u << 10;
+__device__ __forceinline__ bool expires(const KvCacheDev& c) { return c.expire && blockIdx.x + blockIdx.y + blockIdx.z == 0; }
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct AttendDev {

@@ -111,8 +111,7 @@ __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Every wait here is for work of microseconds.
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t phase) { return mbar_wait_polls(bar, phase, 1u << 18); }
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t phase) { return mbar_wait_polls(bar, phase, ATTEND_POLLS); }
 
 // The launch's 512 threads hold 128 registers each; the four warpgroups share
 // them out anew as 192 + 192 + 88 + 40 = 4 x 128.
@@ -167,7 +166,7 @@ struct WideSmem {
   // per key, four tiles deep (a tile's numbers live from its K's loading until
   // its P is done; K of tile j is written once S of tile j - 2 is complete)
   float mul[4][WIDE_KEYS], add[4][WIDE_KEYS], inv[4][WIDE_KEYS];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done, ended, never;
   uint32_t tmem;
   int failed;
 };
@@ -229,6 +228,8 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
       bar_init(smem_u32(&sm.p_full[i]), WIDE_ROWS / 32);
     }
     bar_init(smem_u32(&sm.done), 1);
+    bar_init(smem_u32(&sm.ended), 1);
+    bar_init(smem_u32(&sm.never), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // the query rows; rows past the end are zeros
@@ -255,6 +256,9 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
   fence_after();
   const uint32_t tmem = sm.tmem;
 
+  // A role whose wait runs out ends, and the others' waits for it run out in
+  // their turn; `done` completes only if every product was issued. (A look at
+  // sm.failed in every wait ended all of them at once, and took 5 % of the kernel.)
   bool ok = true;
   if (warp < 8) {
     // ------------------------------------------------------------- softmax
@@ -354,7 +358,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
       warp_arrive(smem_u32(&sm.p_full[slot]));
     }
     if (!ok) sm.failed = 1;
-    if (ok && tiles > 0) ok = __all_sync(FULL, wait(smem_u32(&sm.done), 0));
+    if (ok && tiles > 0) ok = __all_sync(FULL, mbar_wait_polls(smem_u32(&sm.done), 0, ATTEND_POLLS, &sm.failed));
     fence_after();
     // the rows' part; a slot without a key tile of its own has sum 0
     if (ok) {
@@ -387,6 +391,15 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
             for (int x = 0; x < 4; ++x)
               *reinterpret_cast<uint2*>(a.part_o + at[k] * D + c + 8 * x + c2) = make_uint2(o[k >> 1][4 * x + (k & 1) * 2], o[k >> 1][4 * x + (k & 1) * 2 + 1]);
           }
+      }
+    } else {
+      // no part of these rows: their sum is NaN, and so is what it is joined into
+      sm.failed = 1;
+      const int index = parts0 + (pair ? part : 2 * part + slot);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = first + 8 * k;
+        if (r < rows && c2 == 0) a.part_ml[((size_t)index * a.b.rows + token0 + r / a.group) * a.heads + h * a.group + r % a.group] = make_float2(0.0f, NAN);
       }
     }
   } else if (warp < 12) {
@@ -504,6 +517,7 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
         __syncwarp();
       };
       for (int e = 0; e < 2 && e < events; ++e) scores(e);
+      if (expires(a.c)) ok = __all_sync(FULL, mbar_wait_polls(smem_u32(&sm.never), 0, EXPIRE_POLLS));
       for (int e = 0; e < events && ok; ++e) {
         const int slot = e & 1, j = pair ? e >> 1 : e, stage = j & 1;
         ok = __all_sync(FULL, wait(smem_u32(&sm.p_full[slot]), (e >> 1) & 1));
@@ -519,13 +533,13 @@ __global__ void __launch_bounds__(WIDE_ATT_THREADS, 1) k_kv_attend_wide(AttendDe
         __syncwarp();
         if (e + 2 < events) scores(e + 2);
       }
-      if (events > 0) {
+      if (ok && events > 0) {
         if (elect_one()) mma_commit(smem_u32(&sm.done));
+      } else if (events > 0) {
+        sm.failed = 1;
+        if (elect_one()) mma_commit(smem_u32(&sm.ended));
         __syncwarp();
-        if (!ok) {
-          sm.failed = 1;
-          wait(smem_u32(&sm.done), 0);  // what was issued ends before the TMEM is freed
-        }
+        wait(smem_u32(&sm.ended), 0);  // what was issued ends before the TMEM is freed
       }
     }
     __syncwarp();

@@ -4,6 +4,7 @@
 #include <climits>
 #include <string>
 
+#include "../../include/needle_b200_debug.h"
 #include "failure.h"
 #include "serving.h"
 
@@ -232,6 +233,12 @@ nb_status nb_kv_cache_check(nb_kv_cache* cache, void* stream) {
     fail(NB_ERR_ARGUMENT, error & KV_BAD_SEQUENCE ? "a sequence's rows or length were outside the batch's bounds; it was left out"
                                                   : "a page number was outside the pool; its positions were masked or not written");
   });
+}
+
+nb_status nb_debug_expire_attention(nb_kv_cache* cache, uint32_t on) {
+  if (!cache) return NB_ERR_ARGUMENT;
+  cache->dev.expire = on != 0;
+  return NB_OK;
 }
 
 nb_status nb_verify_drafts(int32_t device, const nb_verify* a, void* stream) {

@@ -26,6 +26,7 @@ struct KvCacheDev {
   int kv_heads = 0, dim = 0;
   uint32_t pages = 0;
   bool e4m3 = false;
+  bool expire = false;  // a test's: a wait of the first block of every attention launch runs out
 };
 
 // Rows of 64 codes: eight lanes that read 16 bytes each of two neighbouring

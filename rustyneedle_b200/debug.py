@@ -33,6 +33,7 @@ def _declare() -> None:
         "nb_debug_product": [I, U32, P, P, P, U32, U32, P, U32, P, U32, ctypes.POINTER(ctypes.c_float)],
         "nb_debug_read_bandwidth": [I, SZ, U32, U32, ctypes.POINTER(ctypes.c_float)],
         "nb_debug_expire_waits": [P, U32],
+        "nb_debug_expire_attention": [P, U32],
     }.items():
         fn = getattr(L, name)
         fn.restype = I
@@ -141,3 +142,9 @@ def expire_waits(model: Model, count: int = 1) -> None:
     """The next `count` routing CTAs give up a bounded wait (nb_debug_expire_waits)."""
     _declare()
     _check(lib().nb_debug_expire_waits(model._h, count))
+
+
+def expire_attention(cache, on: bool) -> None:
+    """While it is on, the first blocks of the cache's attention give up a bounded wait (nb_debug_expire_attention)."""
+    _declare()
+    _check(lib().nb_debug_expire_attention(cache._h, int(on)))

@@ -226,3 +226,49 @@ def test_verify_accept_numbers_next_to_their_border(nb, torch, dtype, n, drafts,
     assert want[1][0] == drafts and want[1][1] == 0
     assert np.array_equal(accepted.cpu().numpy(), want[1]), (accepted.cpu().numpy() != want[1]).mean()
     assert np.array_equal(tokens.cpu().numpy(), want[0])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bounds", [{}, {"rows": 8192, "max_rows": 2048, "max_length": 1 << 14}, {"rows": 4000, "max_rows": 150, "max_length": 1 << 17}])
+@pytest.mark.parametrize("prefix, lengths", [(0, [30, 400, 9]), (700, [30, 400, 9]), (5000, [3000, 5, 60])])
+def test_a_wait_of_the_attention_that_runs_out(nb, torch, bounds, dim, prefix, lengths):  # noqa: F811
+    """The first block of every launch gives up: its rows are NaN, the others as they are without it, the call's status is
+    a timeout, once, and the next call is whole again."""
+    from rustyneedle_b200 import debug
+    from tests.test_gpu_serving import int32, make_batch, paged, random_rows
+
+    rng = np.random.default_rng(prefix + dim)
+    kv, heads, rows = 2, 6, [3, 5, 1]
+    prefix_pages, table, pages = paged(rng, lengths, -(-prefix // 64))
+    cache = nb.KvCache(kv, dim, pages, device=0)
+    keys, values = (random_rows(rng, torch, prefix + sum(lengths), kv, dim, torch.bfloat16) for _ in range(2))
+    if prefix:
+        cache.append(make_batch(nb, torch, [prefix], [prefix], prefix_pages[None]), keys[:prefix], values[:prefix])
+    cache.append(make_batch(nb, torch, lengths, lengths, table), keys[prefix:], values[prefix:])
+    query = random_rows(rng, torch, bounds.get("rows", sum(rows)), heads, dim, torch.bfloat16)
+    batch, shared = make_batch(nb, torch, rows, lengths, table, **bounds), int32(torch, prefix_pages)
+
+    def attend():
+        out = torch.full_like(query, 3.0)
+        cache.attend(batch, query, out, shared, prefix)
+        return out
+
+    whole = attend()
+    cache.check()
+    assert bool(torch.isfinite(whole).all())
+    for _ in range(2):
+        debug.expire_attention(cache, True)
+        part = attend()
+        debug.expire_attention(cache, False)
+        with pytest.raises(nb.NeedleError) as e:
+            cache.check()
+        assert e.value.status == -9  # NB_ERR_TIMEOUT
+        cache.check()
+        lost = part.isnan()
+        assert bool(lost[0, : heads // kv].all())  # the first tile is the first sequence's, or the batch's, of the first kv head
+        assert not bool(lost[:, heads // kv :].any())
+        assert torch.equal(torch.where(lost, whole, part), whole)
+        if not prefix:
+            assert not bool(lost[rows[0] :].any())
+        assert torch.equal(attend(), whole)
+        cache.check()
