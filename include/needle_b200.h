@@ -325,7 +325,8 @@ void nb_kv_cache_release(nb_kv_cache* cache);
  * n: row i stands at position lengths[b] - n + i. Position p lies in page
  * pages[b * page_stride + p / NB_KV_PAGE]. rows, max_rows and max_length bound
  * row_start[sequences], n and lengths[b]; they size the launches, so close
- * bounds are faster. The arrays are device memory and may change between
+ * bounds are faster. row_start ascends (where it does not, rows of the other
+ * sequences may be left out as well). The arrays are device memory and may change between
  * replays of a graph, within those bounds. A sequence that breaks a bound
  * (or has lengths[b] < n, or lengths[b] > page_stride * NB_KV_PAGE) is left
  * out: nothing of it is written. A page number outside the pool is neither
@@ -376,7 +377,9 @@ nb_status nb_kv_cache_attend_workspace(const nb_kv_cache* cache, const nb_kv_bat
  * whole batch together, not for each sequence.
  * The tail's new rows have to be in the cache (nb_kv_cache_append, earlier on
  * the same stream). Sums, maxima and products are accumulated in f32; the
- * probabilities enter their product with the codes as f16. `workspace` is
+ * probabilities enter their product with the codes as f16, which is off by
+ * 2^-11 of a probability or 2^-33 of the row's largest probability times value
+ * scale. `workspace` is
  * 16-byte aligned, nb_kv_cache_attend_workspace bytes, free for other use once
  * the call's kernels are done; calls that may overlap (two streams, two graphs)
  * need one each. */

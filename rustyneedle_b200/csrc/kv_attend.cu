@@ -7,7 +7,7 @@
 // so the codes enter both products exactly and every scale stays in f32: the
 // value scale is folded into the exponent, and dividing it out again gives the
 // softmax's own sum. m is the running maximum of t less HEADROOM, so w_j ≤
-// 2^HEADROOM; the product with the codes takes w as f16 (2^-12 relative down
+// 2^HEADROOM; the product with the codes takes w as f16 (2^-11 relative down
 // to 2^-14, absolute 2^-25 below), the sums take it as f32. So the largest p_j
 // vs_j sets the weights' unit: rows of zeros have the smallest scale (a row of
 // zeros of scale 1 with a score 14 above others of 0.02 put 18 % on the result,

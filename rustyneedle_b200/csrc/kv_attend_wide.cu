@@ -30,7 +30,9 @@
 // without the exponentials, the maximum, the weights, the widening, the global
 // loads or one of the two products were 0 to 19% faster each, and one without
 // all of them still took 65 us, the chain of hand-offs from score to weights to
-// product. More slots would fill it, but two have all of TMEM at D = 128;
+// product: a slot's product waits for all weights of a tile, its next scores for
+// the whole product, and the warps that find the maximum also rescale O. More
+// slots would fill it, but two have all of TMEM at D = 128;
 // key tiles of 64 with two score buffers a slot were slower (161 us), as were
 // an issuing warp for each slot (145) and 16 softmax warps (147).
 #include "kv_attend.cuh"
