@@ -390,7 +390,8 @@ nb_status nb_kv_cache_attend(const nb_kv_cache* cache, const nb_kv_batch* batch,
 /* Waits for the stream and reports NB_ERR_ARGUMENT if a call on this cache met
  * a sequence out of its bounds or a page outside the pool since the last
  * check, NB_ERR_TIMEOUT if a bounded device wait gave up (the rows that needed
- * its result are NaN); clears the report. */
+ * its result are NaN). Where several were met it is NB_ERR_TIMEOUT before
+ * NB_ERR_ARGUMENT, and nb_last_error names all. Clears what it reports. */
 nb_status nb_kv_cache_check(nb_kv_cache* cache, void* stream);
 
 /* Drafted tokens against the target model. Sequence b has draft_counts[b]

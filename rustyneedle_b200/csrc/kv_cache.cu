@@ -543,6 +543,15 @@ cudaError_t kv_pool_clear(const KvCacheDev& c, cudaStream_t st) {
   return cudaGetLastError();
 }
 
+// What was reported is taken out of the report word, and no more: kernels of
+// another stream may have added to it meanwhile.
+__global__ void k_kv_clear_report(uint32_t* error, uint32_t reported) { atomicAnd(error, ~reported); }
+
+cudaError_t kv_clear_report(const KvCacheDev& c, uint32_t reported, cudaStream_t st) {
+  k_kv_clear_report<<<1, 1, 0, st>>>(c.error, reported);
+  return cudaGetLastError();
+}
+
 static bool aligned_rows(const RowsDev& r, int size, int n) {
   return reinterpret_cast<uintptr_t>(r.data) % (size * n) == 0 && r.row_stride % n == 0 && r.head_stride % n == 0;
 }

@@ -227,11 +227,16 @@ nb_status nb_kv_cache_check(nb_kv_cache* cache, void* stream) {
     NB_CUDA(cudaMemcpyAsync(&error, cache->dev.error, sizeof error, cudaMemcpyDeviceToHost, st));
     NB_CUDA(cudaStreamSynchronize(st));
     if (!error) return;
-    NB_CUDA(cudaMemsetAsync(cache->dev.error, 0, sizeof error, st));
+    NB_CUDA(kv_clear_report(cache->dev, error, st));
     NB_CUDA(cudaStreamSynchronize(st));
-    if (error & KV_WAIT_FAILED) fail(NB_ERR_TIMEOUT, "a bounded device wait of the shared-prefix attention gave up");
-    fail(NB_ERR_ARGUMENT, error & KV_BAD_SEQUENCE ? "a sequence's rows or length were outside the batch's bounds; it was left out"
-                                                  : "a page number was outside the pool; its positions were masked or not written");
+    std::string message;
+    auto say = [&](uint32_t bit, const char* what) {
+      if (error & bit) message += (message.empty() ? "" : "; ") + std::string(what);
+    };
+    say(KV_WAIT_FAILED, "a bounded device wait of the shared-prefix attention gave up");
+    say(KV_BAD_SEQUENCE, "a sequence's rows or length were outside the batch's bounds, it was left out");
+    say(KV_BAD_PAGE, "a page number was outside the pool, its positions were masked or not written");
+    fail(error & KV_WAIT_FAILED ? NB_ERR_TIMEOUT : NB_ERR_ARGUMENT, message);
   });
 }
 

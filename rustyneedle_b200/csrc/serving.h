@@ -55,6 +55,7 @@ struct RowsDev {
 };
 
 cudaError_t kv_pool_clear(const KvCacheDev& c, cudaStream_t st);
+cudaError_t kv_clear_report(const KvCacheDev& c, uint32_t reported, cudaStream_t st);
 cudaError_t kv_check_spans(const KvCacheDev& c, const KvBatchDev& b, cudaStream_t st);  // for calls without rows
 cudaError_t kv_append(const KvCacheDev& c, const KvBatchDev& b, const RowsDev& keys, const RowsDev& values, cudaStream_t st);
 cudaError_t kv_read(const KvCacheDev& c, const KvBatchDev& b, const RowsDev& keys, const RowsDev& values, cudaStream_t st);

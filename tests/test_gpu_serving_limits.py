@@ -272,3 +272,27 @@ def test_a_wait_of_the_attention_that_runs_out(nb, torch, bounds, dim, prefix, l
             assert not bool(lost[rows[0] :].any())
         assert torch.equal(attend(), whole)
         cache.check()
+
+
+def test_a_report_names_all_that_was_met(nb, torch):  # noqa: F811
+    """A wait that ran out, a sequence out of its bounds and a bad page in one report, none of them lost."""
+    from rustyneedle_b200 import debug
+    from tests.test_gpu_serving import int32, make_batch
+
+    cache = nb.KvCache(2, 64, 4, device=0)
+    x = torch.ones(6, 2, 64, dtype=torch.bfloat16, device="cuda:0")
+    batch = make_batch(nb, torch, [2, 2, 2], [2, 2, 70], np.array([[0, 1], [1, 0], [2, 9]]))
+    bad = make_batch(nb, torch, [2, 2, 2], [2, 1, 70], np.array([[0, 1], [1, 0], [2, 9]]))
+    for first, status, words in ((bad, -9, ["wait", "sequence", "page"]), (batch, -9, ["wait", "page"])):
+        debug.expire_attention(cache, True)
+        cache.attend(first, x, torch.empty_like(x), int32(torch, [3]), 10)
+        debug.expire_attention(cache, False)
+        with pytest.raises(nb.NeedleError) as e:
+            cache.check()
+        assert e.value.status == status and [w for w in ("wait", "sequence", "page") if w in e.value.message] == words
+        cache.check()
+    cache.append(bad, x, x)
+    with pytest.raises(nb.NeedleError) as e:
+        cache.check()
+    assert e.value.status == -4 and "sequence" in e.value.message and "page" in e.value.message
+    cache.check()
