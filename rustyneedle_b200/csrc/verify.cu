@@ -111,8 +111,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// 2^(y / 128) for -128000 <= y <= 0 in f64: y = k + f, k whole, |f| <= 1/2; the
-// table holds 2^(j / 128), sixteen times over so that no two lanes of a half
+// 2^(y / 128) for -128000 <= y <= 0 in f64, a table-driven exponential after
+// P. T. P. Tang (1989): y = k + f, k whole, |f| <= 1/2; the table holds 2^(j / 128), sixteen times over so that no two lanes of a half
 // warp meet in a bank, and 2^(f / 128) = e^r with r = f ln2 / 128 (|r| <=
 // 0.0028) is its Taylor polynomial of degree 3, within 3e-12 relative. The
 // power of two goes into the table's value: 2^(y / 128) = e · t. Entry j's high
